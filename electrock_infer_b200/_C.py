@@ -33,6 +33,15 @@ def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def _call(dev: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on the current stream of ``dev``, with ``dev`` current.  Decode-step ops
+    take microseconds on the device, so the guard is entered only when another device is current."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
 def _float_tag(name: str, t: torch.Tensor) -> int:
     try:
         return _FLOAT_TAGS[t.dtype]
@@ -358,6 +367,185 @@ def paged_attn_varlen(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Ten
             block_table.data_ptr(), context_lens.data_ptr(), tag, batch, q_heads, kv_heads,
             head_dim, num_blocks, block_size, max_blocks, float(softmax_scale), num_splits,
             ws_ptr, ws_bytes, _stream(dev))
+    _lib.check(rc, name)
+    _lib.count_launches(2 if num_splits > 1 else 1)
+    return out
+
+
+def paged_schedule_max_requests() -> int:
+    """Most requests that one ``paged_schedule`` call takes."""
+    return _lib.load().b200moe_paged_schedule_max_requests()
+
+
+def paged_schedule(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                   free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int,
+                   seq_lens: torch.Tensor, cu_seqlens: torch.Tensor, slot_mapping: torch.Tensor,
+                   positions: torch.Tensor | None, free_count_out: torch.Tensor,
+                   num_refused: torch.Tensor) -> None:
+    """Builds the tables of one step on the GPU from the requests' lengths: what the reference's host
+    loop (engine/model_runner.py, prepare_prefill / prepare_decode, and engine/block_manager.py) fills
+    page by page before every step.
+
+    ``context_lens`` i32 ``[R]``: tokens of request i in the cache.  ``new_lens`` i32 ``[R]``: token rows
+    it brings this step; 0 waits, a negative value ends the request.  ``block_table`` i32
+    ``[R, max_blocks]`` (row stride free): pages of each request, in order; entries past a request's
+    length mean nothing.  ``free_blocks`` i32: a stack whose first ``free_count[0]`` entries are the free
+    pages; it should have room for every page of the cache (pages pushed beyond it are lost).
+
+    Ended requests push their pages in request order; then the others pop the pages they lack, in
+    request order, from the top.  A request is refused, and keeps its length, when its table row is too
+    short, when its rows lie beyond ``slot_mapping``, or when it needs pages and they, with those of all
+    requests before it, are more than there are.  Outputs, all overwritten:
+
+    ``seq_lens`` i32 ``[R]`` lengths after the step (0 for ended requests; may be ``context_lens``),
+    ``cu_seqlens`` i32 ``[R + 1]`` first row of each request, ``slot_mapping`` i32 ``[N]`` cache slot of
+    each row (-1 for rows of refused requests and for rows behind the last request, which the store ops
+    skip), ``positions`` i64 ``[N]`` or None (0 behind the last request), ``free_count_out`` i32 ``[1]``
+    (may be ``free_count``), ``num_refused`` i32 ``[1]``.  New entries are written into ``block_table`` and
+    pushed pages into ``free_blocks``.  Apart from the two pairs named, no tensors may overlap.
+    """
+    name = "paged_schedule"
+    tensors = [context_lens, new_lens, free_blocks, free_count, seq_lens, cu_seqlens, slot_mapping,
+               free_count_out, num_refused]
+    dev = _require_cuda(name, *tensors)
+    for t in tensors:
+        if t.dtype != torch.int32:
+            raise RuntimeError(f"{name}: lengths, pages and slots must be int32, got {t.dtype}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev:
+        raise RuntimeError(f"{name}: block_table must be int32 [requests, max_blocks] on {dev}")
+    requests, max_blocks = block_table.shape
+    if max_blocks and block_table.stride(1) != 1:
+        raise RuntimeError(f"{name}: the entries of a block_table row must be contiguous")
+    if (context_lens.numel() != requests or new_lens.numel() != requests
+            or seq_lens.numel() != requests or cu_seqlens.numel() != requests + 1):
+        raise RuntimeError(f"{name}: context_lens, new_lens and seq_lens must hold {requests} elements "
+                           f"and cu_seqlens {requests + 1}")
+    if free_count.numel() != 1 or free_count_out.numel() != 1 or num_refused.numel() != 1:
+        raise RuntimeError(f"{name}: free_count, free_count_out and num_refused hold one element")
+    rows = slot_mapping.numel()
+    if positions is not None and (positions.dtype != torch.int64 or positions.numel() != rows
+                                  or positions.device != dev or not positions.is_contiguous()):
+        raise RuntimeError(f"{name}: positions must be contiguous int64 with one entry per row of slot_mapping")
+    rc = _call(dev, _lib.load().b200moe_paged_schedule,
+               context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+               free_blocks.data_ptr(), free_count.data_ptr(), requests, max_blocks,
+               block_table.stride(0) if requests > 1 else max_blocks, block_size,
+               free_blocks.numel(), rows, seq_lens.data_ptr(), cu_seqlens.data_ptr(),
+               slot_mapping.data_ptr(), positions.data_ptr() if positions is not None else None,
+               free_count_out.data_ptr(), num_refused.data_ptr())
+    _lib.check(rc, name)
+    _lib.count_launches(1)
+
+
+def _check_codes(name: str, K_cache: torch.Tensor, V_cache: torch.Tensor,  # noqa: N803
+                 K_scale: torch.Tensor, V_scale: torch.Tensor) -> None:  # noqa: N803
+    if K_cache.dim() != 4 or V_cache.shape != K_cache.shape:
+        raise RuntimeError(f"{name}: caches must both be [blocks, block_size, kv_heads, head_dim]")
+    if K_cache.dtype != torch.float8_e4m3fn or V_cache.dtype != torch.float8_e4m3fn:
+        raise RuntimeError(f"{name}: caches must be float8_e4m3fn, got {K_cache.dtype} and {V_cache.dtype}")
+    shape = (K_cache.size(0), K_cache.size(2))
+    if (K_scale.dtype != torch.float32 or V_scale.dtype != torch.float32 or K_scale.shape != shape
+            or V_scale.shape != shape):
+        raise RuntimeError(f"{name}: scales must be float32 [blocks, kv_heads] = {list(shape)}")
+
+
+def paged_store_kvcache_fp8(K: torch.Tensor, V: torch.Tensor, K_cache: torch.Tensor,  # noqa: N803
+                            V_cache: torch.Tensor, K_scale: torch.Tensor, V_scale: torch.Tensor,  # noqa: N803
+                            slot_mapping: torch.Tensor) -> None:
+    """``paged_store_kvcache`` into caches held in 8 bits (no counterpart in the reference, whose
+    caches hold the model's element type).
+
+    ``K``, ``V`` ``[tokens, kv_heads, 128]`` bf16, fp16 or fp32 (the token stride may exceed a row);
+    caches ``float8_e4m3fn [blocks, block_size, kv_heads, 128]``; scales float32 ``[blocks, kv_heads]``,
+    zero for pages that were never stored to; ``slot_mapping`` int32 ``[tokens]``.  Negative slots and
+    slots beyond the cache are skipped.
+
+    A stored value is ``code * scale`` with one scale per page and head, a power of two between 2^-32
+    and 2^32: the smallest that brings every finite value the page has received within e4m3's 448.  When a
+    call raises a page's scale, its old codes are rounded again under the new one.  A call that stores to
+    a page's first slot begins that page anew: what it held, and its scale, count for nothing.  NaN is
+    stored as NaN, infinities and values out of range as the largest code of their sign.
+
+    Slots must be distinct, and the tokens of one page must follow one another in the call with nothing
+    but skipped entries between them, as in every slot map that is built request by request.
+    """
+    name = "paged_store_kvcache_fp8"
+    dev = _require_cuda(name, K_cache, V_cache, K_scale, V_scale, slot_mapping)
+    _check_codes(name, K_cache, V_cache, K_scale, V_scale)
+    num_blocks, block_size, kv_heads, head_dim = K_cache.shape
+    if K.dim() != 3 or V.shape != K.shape or K.size(1) != kv_heads or K.size(2) != head_dim:
+        raise RuntimeError(f"{name}: K and V must both be [tokens, {kv_heads}, {head_dim}]")
+    if K.device != dev or V.device != dev:
+        raise RuntimeError(f"{name}: K and V must be on {dev}, like the caches")
+    if K.dtype != V.dtype:
+        raise RuntimeError(f"{name}: K and V must share a dtype")
+    num_tokens = K.size(0)
+    for t in (K, V):
+        if t.stride(2) != 1 or (kv_heads > 1 and t.stride(1) != head_dim):
+            raise RuntimeError(f"{name}: the heads of a token must be contiguous")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != num_tokens:
+        raise RuntimeError(f"{name}: slot_mapping must be int32 with one entry per token")
+    row = kv_heads * head_dim
+    rc = _call(dev, _lib.load().b200moe_paged_store_kvcache_fp8,
+               K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), K_scale.data_ptr(),
+               V_scale.data_ptr(), slot_mapping.data_ptr(), _float_tag(name, K), num_tokens, kv_heads,
+               head_dim, K.stride(0) if num_tokens > 1 else row, V.stride(0) if num_tokens > 1 else row,
+               num_blocks, block_size)
+    _lib.check(rc, name)
+    _lib.count_launches(1 if num_tokens else 0)
+
+
+def paged_attn_varlen_fp8(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor,  # noqa: N803
+                          K_scale: torch.Tensor, V_scale: torch.Tensor, max_seqlen_k: int,  # noqa: N803
+                          context_lens: torch.Tensor, block_table: torch.Tensor, softmax_scale: float,
+                          num_splits: int = 0) -> torch.Tensor:
+    """``paged_attn_varlen`` over caches held in 8 bits, as ``paged_store_kvcache_fp8`` fills them (no
+    counterpart in the reference).  Returns a new contiguous ``O [batch, q_heads, 128]``.
+
+    ``Q`` bf16 or fp16 ``[batch, q_heads, 128]`` (the batch stride may exceed a row); caches, scales as
+    in the store; ``context_lens`` int32 ``[batch]``; ``block_table`` int32 ``[batch, max_blocks]`` (row
+    stride free).  Up to 16 query heads per KV head, block sizes that are multiples of 16.  An empty
+    context gives a zero row.  ``max_seqlen_k`` (0 = unknown) only helps to choose ``num_splits`` (0 =
+    choose), the number of ranges that a context is cut into.  The scratch of the merge is allocated per
+    call from torch's allocator, so that calls on different streams and captured graphs never share it.
+    """
+    name = "paged_attn_varlen_fp8"
+    dev = _require_cuda(name, K_cache, V_cache, K_scale, V_scale, context_lens)
+    _check_codes(name, K_cache, V_cache, K_scale, V_scale)
+    num_blocks, block_size, kv_heads, head_dim = K_cache.shape
+    if Q.dim() != 3 or Q.size(2) != head_dim:
+        raise RuntimeError(f"{name}: Q must be [batch, heads, {head_dim}]")
+    batch, q_heads, _ = Q.shape
+    if Q.device != dev or block_table.device != dev:
+        raise RuntimeError(f"{name}: Q and block_table must be on {dev}, like the caches")
+    if Q.stride(2) != 1 or (q_heads > 1 and Q.stride(1) != head_dim):
+        raise RuntimeError(f"{name}: the heads of a query must be contiguous")
+    if context_lens.dtype != torch.int32 or block_table.dtype != torch.int32:
+        raise RuntimeError(f"{name}: context_lens and block_table must be int32")
+    if block_table.dim() != 2 or block_table.size(0) != batch or context_lens.numel() != batch:
+        raise RuntimeError(f"{name}: block_table must be [batch, max_blocks] and context_lens [batch]")
+    max_blocks = block_table.size(1)
+    if max_blocks > 1 and block_table.stride(1) != 1:
+        raise RuntimeError(f"{name}: the entries of a block_table row must be contiguous")
+    tag = _float_tag(name, Q)
+    lib = _lib.load()
+    out = torch.empty((batch, q_heads, head_dim), dtype=Q.dtype, device=dev)
+    if num_splits <= 0:
+        longest = max_blocks * block_size
+        if 0 < max_seqlen_k < longest:
+            longest = max_seqlen_k
+        num_splits = lib.b200moe_paged_attn_fp8_num_splits(batch, kv_heads, longest)
+    ws, ws_ptr, ws_bytes = None, None, 0
+    if num_splits > 1:
+        ws_bytes = lib.b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_ptr = ws.data_ptr()
+    rc = _call(dev, lib.b200moe_paged_attn_varlen_fp8,
+               Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), K_scale.data_ptr(),
+               V_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), tag,
+               batch, q_heads, kv_heads, head_dim, Q.stride(0) if batch > 1 else q_heads * head_dim,
+               num_blocks, block_size, max_blocks, block_table.stride(0) if batch > 1 else max_blocks,
+               float(softmax_scale), num_splits, ws_ptr, ws_bytes)
     _lib.check(rc, name)
     _lib.count_launches(2 if num_splits > 1 else 1)
     return out

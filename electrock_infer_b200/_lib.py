@@ -67,6 +67,19 @@ SIGNATURES = {
     "b200moe_paged_attn_varlen": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                           c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int,
                                           c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "b200moe_paged_store_kvcache_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                c_void_p, c_int, c_int64, c_int, c_int, c_int64, c_int64,
+                                                c_int64, c_int, c_void_p]),
+    "b200moe_paged_attn_fp8_num_splits": (c_int, [c_int, c_int, c_int64]),
+    "b200moe_paged_attn_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "b200moe_paged_attn_varlen_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                              c_int64, c_int64, c_int, c_int, c_int64, c_float, c_int,
+                                              c_void_p, c_size_t, c_void_p]),
+    "b200moe_paged_schedule_max_requests": (c_int, []),
+    "b200moe_paged_schedule": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                       c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p]),
     "b200moe_peer_alloc": (c_int, [c_size_t, ctypes.POINTER(c_void_p), c_void_p]),
     "b200moe_peer_open": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "b200moe_peer_close": (c_int, [c_void_p]),

@@ -1,0 +1,490 @@
+// Decode attention over the 8-bit paged cache: one query token per sequence, grouped query heads.
+//
+//   q, out            [batch, q_heads, 128] bf16 or fp16 (q rows may be strided)
+//   k_cache, v_cache  [num_blocks, block_size, kv_heads, 128] e4m3 codes
+//   k_scale, v_scale  [num_blocks, kv_heads] fp32, value = code * scale
+//   block_table       [batch, max_blocks] int32, context_lens [batch] int32
+//   out[b, h] = softmax(scale * q[b, h] . K[b, h / group, :ctx]) @ V[b, h / group, :ctx]
+//
+// The reference has no 8-bit cache; its kernel (src/paged_attn_gqa_varlen.hip:17-213) streams a 16-bit
+// one once per QUERY head.  Half the bytes per token also means half the time per token, so what
+// the 16-bit kernel of this library spends per token beside its loads is too much here.  Both products
+// are therefore taken transposed:
+//
+//   S^T = K q^T   16 tokens x 8 heads, A = codes of K widened to fp16 in registers, B = q^T
+//   O^T = V^T P^T 16 dims x 8 heads,   A = codes of V widened to fp16, B = P^T
+//
+// with m16n8k16: the tile is 8 heads wide, not 16 rows high, so groups of up to 8 query heads cost half
+// the tensor instructions, exponentials and accumulators of a 16-row query tile (groups of 9 to 16 take
+// two such tiles).  Fragments come from 16-byte shared-memory reads, not from matrix loads: the
+// contraction index of S and the output rows of O may be permuted at will, so a lane takes 16
+// consecutive codes of its token and the query is laid out to match; V's pairs of neighbouring tokens
+// are interleaved by byte permutes before they are widened.  fp16 holds every e4m3 value exactly, so
+// widening rounds nothing; q rows are scaled by a power of two into fp16's range (exact for
+// fp16 and bf16 values within 2^-38 of the row's largest), P is rounded to fp16 (2^-12 relative, below
+// the rounding of the output), all sums, maxima and the outputs are fp32.
+//
+// Four warps stream their own 32-token chunks through a three-stage ring of asynchronous 16-byte copies
+// (rows of 128 bytes, XOR-swizzled).  A page's K scale multiplies the scores; its V scale is the unit that
+// the accumulators are kept in, which is exchanged only where a warp comes to another page.  With
+// num_splits > 1 the context is cut into ranges for separate CTAs and a second kernel merges them.
+// Bound by HBM: 256 bytes per token and KV head.
+#include "fp8_cache.cuh"
+#include "warp_mma.cuh"
+
+namespace b200moe {
+namespace {
+
+constexpr int kDim = kCodeHeadDim;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16;                  // tokens of one product; a tile never crosses a page
+constexpr int kChunkTiles = 2;             // tiles per ring stage
+constexpr int kChunk = kTile * kChunkTiles;
+constexpr int kStages = 3;
+constexpr int kHalfBytes = kChunk * kDim;  // 4 KiB of K, as much of V
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kRingBytes = kWarps * kStages * kStageBytes;                    // 96 KiB
+constexpr int kScaleBytes = kWarps * kStages * 2 * kChunkTiles * sizeof(float);
+constexpr int kSmemBytes = kRingBytes + kScaleBytes;                          // two CTAs per SM
+constexpr int kMaxGroup = 16;
+constexpr int kMaxContext = 0x7fffffff - 2 * kChunk;  // so that rounding up to chunks stays in range
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  const void* q;
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  void* out;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  float* ws_o;   // [batch, q_heads, splits, 128] un-normalised partial outputs
+  float* ws_ml;  // [batch, q_heads, splits, 2] running max (log2 domain) and sum
+  int64_t q_stride, num_blocks, table_stride;
+  int q_heads, kv_heads, group, block_size, max_blocks, num_splits;
+  float scale_log2;
+};
+
+// Byte offset of 16-byte column `col` of token row `row` in a swizzled tile of 128-byte rows.
+__device__ __forceinline__ uint32_t tile_offset(int row, int col) {
+  return static_cast<uint32_t>(row * kDim + ((col ^ (row & 7)) << 4));
+}
+
+template <typename T, int kNT>  // kNT = tiles of 8 query heads
+__global__ void __launch_bounds__(kThreads, 2)
+paged_attn_fp8_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % p.num_splits;
+  const int kvh = (blockIdx.x / p.num_splits) % p.kv_heads;
+  const int seq = blockIdx.x / (p.num_splits * p.kv_heads);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // A context never reaches past the pages the table row can name.
+  const int ctx = static_cast<int>(min(static_cast<int64_t>(min(max(p.context_lens[seq], 0), kMaxContext)),
+                                       static_cast<int64_t>(p.max_blocks) * p.block_size));
+  int per_split = (ctx - 1) / p.num_splits + 1;
+  per_split = ((per_split - 1) / kChunk + 1) * kChunk;
+  const int t_begin = static_cast<int>(min(static_cast<int64_t>(split) * per_split, static_cast<int64_t>(ctx)));
+  const int t_end = per_split < ctx - t_begin ? t_begin + per_split : ctx;
+  const int num_chunks = (t_end - t_begin + kChunk - 1) / kChunk;
+
+  const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
+  float* scales = reinterpret_cast<float*>(smem + kRingBytes) + warp * kStages * 2 * kChunkTiles;
+  const uint32_t scales_addr = smem_addr(scales);
+  const int32_t* table = p.block_table + seq * p.table_stride;
+  const int64_t row_bytes = static_cast<int64_t>(p.kv_heads) * kDim;
+
+  // Issues the copies of the CTA's chunk `ci` into ring slot `stage`.  A page outside the cache is
+  // replaced by page 0, tokens past the range are filled with zeros (0 * NaN would poison the output).
+  auto issue = [&](int ci, int stage) {
+    if (ci < num_chunks) {
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile) {
+        const int tok = t_begin + ci * kChunk + tile * kTile;
+        int page = 0, off = 0;
+        if (tok < t_end) {
+          page = table[tok / p.block_size];
+          off = tok % p.block_size;
+          if (page < 0 || page >= p.num_blocks) page = 0;
+        }
+        const int row = lane >> 3, col = lane & 7;
+        const int64_t at = (static_cast<int64_t>(page) * p.block_size + off + (tok < t_end ? row : 0)) * row_bytes +
+                           kvh * kDim + col * 16;
+        const uint32_t dst = ring + stage * kStageBytes + tile * kTile * kDim;
+#pragma unroll
+        for (int j = 0; j < kTile / 4; ++j) {
+          const int bytes = tok + row + j * 4 < t_end ? 16 : 0;
+          const int64_t from = at + (bytes ? j * 4 * row_bytes : 0);
+          const uint32_t to = dst + tile_offset(row + j * 4, col);
+          cp_async_16(to, p.k_cache + from, bytes);
+          cp_async_16(to + kHalfBytes, p.v_cache + from, bytes);
+        }
+        if (lane < 2) {
+          const float* s = (lane ? p.v_scale : p.k_scale) + static_cast<int64_t>(page) * p.kv_heads + kvh;
+          cp_async_4(scales_addr + (stage * 2 * kChunkTiles + tile * 2 + lane) * 4, s);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+
+  // Warp w owns chunks w, w + 4, w + 8, ... of the CTA's range.
+  const int my_chunks = num_chunks > warp ? (num_chunks - warp + kWarps - 1) / kWarps : 0;
+  auto chunk_index = [&](int i) { return i < my_chunks ? warp + i * kWarps : num_chunks; };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) issue(chunk_index(s), s);
+
+  // Query rows as B fragments: column n = head, and the contraction index of step 4 * i + w in lane t
+  // is the dims (2 t + i) * 16 + 4 w .. + 3, the order in which the lane reads its tokens' codes.
+  uint32_t qb[kNT][kDim / 16][2];
+  float qmul[kNT][2];  // score factor of heads 2 t and 2 t + 1 (the columns of a lane's accumulators)
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const bool live = n * 8 + g < p.group;
+    const T* q = static_cast<const T*>(p.q) + seq * p.q_stride +
+                 (static_cast<int64_t>(kvh) * p.group + (live ? n * 8 + g : 0)) * kDim;
+    float x[2][16];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 v = live ? *reinterpret_cast<const uint4*>(q + (2 * t + i) * 16 + h * 8) : make_uint4(0, 0, 0, 0);
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[i][h * 8 + j] = Mma<T>::to_float(e[j]);
+          const uint32_t b = __float_as_uint(x[i][h * 8 + j]) & 0x7fffffffu;
+          amax = max(amax, b < 0x7f800000u ? b : 0u);
+        }
+      }
+    }
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // 2^up brings the row's largest value to [2^14, 2^15).
+    const int up = amax >> 23 ? min(max(14 + 127 - static_cast<int>(amax >> 23), -126), 126) : 0;
+    const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    const float back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    qmul[n][0] = __shfl_sync(0xffffffffu, back, 8 * t) * p.scale_log2;
+    qmul[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * p.scale_log2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        qb[n][i * 4 + w][0] = Mma<__half>::pack(x[i][4 * w] * f, x[i][4 * w + 1] * f);
+        qb[n][i * 4 + w][1] = Mma<__half>::pack(x[i][4 * w + 2] * f, x[i][4 * w + 3] * f);
+      }
+  }
+
+  // o[n][m]: dims g * 16 + 2 m (elements 0, 1) and g * 16 + 2 m + 1 (2, 3) of heads 2 t and 2 t + 1.
+  float o[kNT][kDim / 16][4];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int m = 0; m < kDim / 16; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[n][m][j] = 0.f;
+  float mx[kNT][2], sum[kNT][2];  // running maximum; this lane's part of the sum
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    mx[n][0] = mx[n][1] = -INFINITY;
+    sum[n][0] = sum[n][1] = 0.f;
+  }
+  float unit = 1.f;  // V scale that o is expressed in
+
+  for (int i = 0; i < my_chunks; ++i) {
+    const int stage = i % kStages;
+    issue(chunk_index(i + kStages - 1), (i + kStages - 1) % kStages);
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t ksm = ring + stage * kStageBytes, vsm = ksm + kHalfBytes;
+    const float* sc = scales + stage * 2 * kChunkTiles;
+    const int tok0 = t_begin + (warp + i * kWarps) * kChunk;
+
+    float s[kChunkTiles][kNT][4];
+#pragma unroll
+    for (int tile = 0; tile < kChunkTiles; ++tile) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[tile][n][j] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 lo = lds_16(ksm + tile_offset(tile * kTile + g, 2 * t + h));
+        const uint4 hi = lds_16(ksm + tile_offset(tile * kTile + g + 8, 2 * t + h));
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t a[4] = {codes_to_half2(wl[w] & 0xffffu), codes_to_half2(wh[w] & 0xffffu),
+                                 codes_to_half2(wl[w] >> 16), codes_to_half2(wh[w] >> 16)};
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) Mma<__half>::run(s[tile][n], a, qb[n][h * 4 + w][0], qb[n][h * 4 + w][1]);
+        }
+      }
+      // Into the exp2 domain; tokens past the range do not count.
+      const float ks = usable_scale(sc[tile * 2]);
+      const bool v0 = tok0 + tile * kTile + g < t_end, v1 = tok0 + tile * kTile + g + 8 < t_end;
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        s[tile][n][0] = v0 ? s[tile][n][0] * (qmul[n][0] * ks) : -INFINITY;
+        s[tile][n][1] = v0 ? s[tile][n][1] * (qmul[n][1] * ks) : -INFINITY;
+        s[tile][n][2] = v1 ? s[tile][n][2] * (qmul[n][0] * ks) : -INFINITY;
+        s[tile][n][3] = v1 ? s[tile][n][3] * (qmul[n][1] * ks) : -INFINITY;
+      }
+    }
+    // A chunk holds at least one token of the range, so the new maxima are finite.
+    uint32_t pb[kChunkTiles][kNT][2];  // P^T as B fragments
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      float alpha[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+        for (int tile = 1; tile < kChunkTiles; ++tile) top = fmaxf(top, fmaxf(s[tile][n][c], s[tile][n][c + 2]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        top = fmaxf(top, mx[n][c]);
+        alpha[c] = exp2f(mx[n][c] - top);  // exp2(-inf) = 0 on the first chunk
+        mx[n][c] = top;
+        sum[n][c] *= alpha[c];
+#pragma unroll
+        for (int tile = 0; tile < kChunkTiles; ++tile) {
+          s[tile][n][c] = exp2f(s[tile][n][c] - top);
+          s[tile][n][c + 2] = exp2f(s[tile][n][c + 2] - top);
+          sum[n][c] += s[tile][n][c] + s[tile][n][c + 2];
+        }
+      }
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile) {
+        pb[tile][n][0] = transpose_8x8(Mma<__half>::pack(s[tile][n][0], s[tile][n][1]));
+        pb[tile][n][1] = transpose_8x8(Mma<__half>::pack(s[tile][n][2], s[tile][n][3]));
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int m = 0; m < kDim / 16; ++m) {
+          o[n][m][0] *= alpha[0]; o[n][m][1] *= alpha[1];
+          o[n][m][2] *= alpha[0]; o[n][m][3] *= alpha[1];
+        }
+      }
+    }
+#pragma unroll
+    for (int tile = 0; tile < kChunkTiles; ++tile) {
+      const float vs = usable_scale(sc[tile * 2 + 1]);
+      if (vs != unit && tok0 + tile * kTile < t_end) {
+        const float f = unit / vs;
+        unit = vs;
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int m = 0; m < kDim / 16; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][m][j] *= f;
+      }
+      uint32_t w[4][4];  // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the tile, 16 dims each
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint4 v = lds_16(vsm + tile_offset(tile * kTile + 2 * t + (r & 1) + (r >> 1) * 8, g));
+        w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // Bytes of two tokens interleaved: each half is one dim's pair.
+        const uint32_t lo0 = __byte_perm(w[0][q], w[1][q], 0x5140), lo1 = __byte_perm(w[0][q], w[1][q], 0x7362);
+        const uint32_t hi0 = __byte_perm(w[2][q], w[3][q], 0x5140), hi1 = __byte_perm(w[2][q], w[3][q], 0x7362);
+        const uint32_t a0[4] = {codes_to_half2(lo0 & 0xffffu), codes_to_half2(lo0 >> 16),
+                                codes_to_half2(hi0 & 0xffffu), codes_to_half2(hi0 >> 16)};
+        const uint32_t a1[4] = {codes_to_half2(lo1 & 0xffffu), codes_to_half2(lo1 >> 16),
+                                codes_to_half2(hi1 & 0xffffu), codes_to_half2(hi1 >> 16)};
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          Mma<__half>::run(o[n][2 * q], a0, pb[tile][n][0], pb[tile][n][1]);
+          Mma<__half>::run(o[n][2 * q + 1], a1, pb[tile][n][0], pb[tile][n][1]);
+        }
+      }
+    }
+    __syncwarp();  // the slot is refilled by the next iteration's copies
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // Merge the four warps through shared memory (the ring is free now).
+  float* sm_o = reinterpret_cast<float*>(smem);          // [warps][kNT * 8][128]
+  float* sm_ml = sm_o + kWarps * kNT * 8 * kDim;         // [warps][kNT * 8][2]
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = sum[n][c];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int row = warp * kNT * 8 + n * 8 + 2 * t + c;
+      float* wo = sm_o + row * kDim + g * 16;
+#pragma unroll
+      for (int m = 0; m < kDim / 16; ++m)
+        *reinterpret_cast<float2*>(wo + 2 * m) = make_float2(o[n][m][c] * unit, o[n][m][c + 2] * unit);
+      if (g == 0) {
+        sm_ml[row * 2] = mx[n][c];
+        sm_ml[row * 2 + 1] = l;
+      }
+    }
+  }
+  __syncthreads();
+  // Thread d owns output dimension d for every head of the group.
+  const int d = threadIdx.x;
+  for (int r = 0; r < p.group; ++r) {
+    float mw[kWarps], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mw[w] = sm_ml[(w * kNT * 8 + r) * 2];
+      top = fmaxf(top, mw[w]);
+    }
+    float l = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float lw = sm_ml[(w * kNT * 8 + r) * 2 + 1];
+      const float f = lw == 0.f ? 0.f : exp2f(mw[w] - top);  // a warp without tokens has sum 0
+      l += f * lw;
+      acc += f * sm_o[(w * kNT * 8 + r) * kDim + d];
+    }
+    const int64_t head = static_cast<int64_t>(seq) * p.q_heads + static_cast<int64_t>(kvh) * p.group + r;
+    if (p.num_splits == 1) {
+      // An empty context gives zeros (the reference divides 0 by 0 there).
+      static_cast<T*>(p.out)[head * kDim + d] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
+    } else {
+      p.ws_o[(head * p.num_splits + split) * kDim + d] = acc;
+      if (d == 0) {
+        p.ws_ml[(head * p.num_splits + split) * 2] = top;
+        p.ws_ml[(head * p.num_splits + split) * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+// Merges the splits of one (sequence, query head): thread d owns dimension d.
+template <typename T>
+__global__ void __launch_bounds__(kDim)
+paged_attn_fp8_merge_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
+                            T* __restrict__ out, int num_splits) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t head = blockIdx.x;
+  const int d = threadIdx.x;
+  float top = -INFINITY;
+  for (int s = 0; s < num_splits; ++s) top = fmaxf(top, ws_ml[(head * num_splits + s) * 2]);
+  float l = 0.f, acc = 0.f;
+  for (int s = 0; s < num_splits; ++s) {
+    const float ls = ws_ml[(head * num_splits + s) * 2 + 1];
+    const float f = ls == 0.f ? 0.f : exp2f(ws_ml[(head * num_splits + s) * 2] - top);
+    l += f * ls;
+    acc += f * ws_o[(head * num_splits + s) * kDim + d];
+  }
+  out[head * kDim + d] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
+}
+
+template <typename T, int kNT>
+int launch(const Params& p, int batch, cudaStream_t st) {
+  // Per device and per function; cheap enough to repeat on every call.
+  const cudaError_t e = cudaFuncSetAttribute(
+      paged_attn_fp8_kernel<T, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "paged_attn_varlen_fp8: %s", cudaGetErrorString(e));
+  const int64_t ctas = static_cast<int64_t>(batch) * p.kv_heads * p.num_splits;
+  launch_pdl(paged_attn_fp8_kernel<T, kNT>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmemBytes, st, p);
+  if (int rc = check_launch("paged_attn_varlen_fp8")) return rc;
+  if (p.num_splits > 1) {
+    launch_pdl(paged_attn_fp8_merge_kernel<T>, dim3(static_cast<unsigned>(batch * p.q_heads)), dim3(kDim), 0, st,
+               static_cast<const float*>(p.ws_o), static_cast<const float*>(p.ws_ml), static_cast<T*>(p.out),
+               p.num_splits);
+    return check_launch("paged_attn_varlen_fp8 (merge)");
+  }
+  return B200MOE_OK;
+}
+
+constexpr int kMaxSplits = 64;
+
+}  // namespace
+}  // namespace b200moe
+
+extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int kv_heads, int64_t max_context) {
+  using namespace b200moe;
+  if (batch < 1 || kv_heads < 1 || max_context < 1) return 1;
+  const int64_t ctas = static_cast<int64_t>(batch) * kv_heads;
+  const int64_t want = ceil_div64(6ll * sm_count(), ctas);
+  const int64_t by_length = max_context / 512 > 0 ? max_context / 512 : 1;
+  int64_t s = want < by_length ? want : by_length;
+  if (s < 1) s = 1;
+  if (s > kMaxSplits) s = kMaxSplits;
+  return static_cast<int>(s);
+}
+
+extern "C" size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int num_splits) {
+  if (batch < 1 || q_heads < 1 || num_splits <= 1) return 0;
+  return static_cast<size_t>(batch) * q_heads * num_splits * (b200moe::kDim + 2) * sizeof(float);
+}
+
+extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache, const void* v_cache,
+                                             const float* k_scale, const float* v_scale, void* out,
+                                             const int32_t* block_table, const int32_t* context_lens,
+                                             int dtype, int batch, int q_heads, int kv_heads,
+                                             int head_dim, int64_t q_row_stride, int64_t num_blocks,
+                                             int block_size, int max_blocks_per_seq,
+                                             int64_t table_row_stride, float softmax_scale,
+                                             int num_splits, void* workspace, size_t workspace_bytes,
+                                             b200moe_stream_t stream) {
+  using namespace b200moe;
+  const char* name = "paged_attn_varlen_fp8";
+  if (dtype != B200MOE_BF16 && dtype != B200MOE_F16)
+    return fail(B200MOE_ERR_DTYPE, "%s: bf16 or fp16 queries only, got dtype %d", name, dtype);
+  if (head_dim != kDim) return fail(B200MOE_ERR_SHAPE, "%s: head_dim must be 128, got %d", name, head_dim);
+  if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0)
+    return fail(B200MOE_ERR_SHAPE, "%s: batch=%d q_heads=%d kv_heads=%d (q_heads must be a multiple "
+                "of kv_heads)", name, batch, q_heads, kv_heads);
+  const int group = q_heads / kv_heads;
+  if (group > kMaxGroup)
+    return fail(B200MOE_ERR_UNSUPPORTED, "%s: at most %d query heads per KV head, got %d", name,
+                kMaxGroup, group);
+  if (block_size < kTile || block_size % kTile != 0)
+    return fail(B200MOE_ERR_SHAPE, "%s: block_size must be a multiple of %d, got %d", name, kTile, block_size);
+  if (num_blocks < 1 || num_blocks > 0x7fffffffLL || max_blocks_per_seq < 1 ||
+      table_row_stride < max_blocks_per_seq || num_splits < 1 || num_splits > kMaxSplits)
+    return fail(B200MOE_ERR_SHAPE, "%s: num_blocks=%lld max_blocks_per_seq=%d (row stride %lld) num_splits=%d",
+                name, (long long)num_blocks, max_blocks_per_seq, (long long)table_row_stride, num_splits);
+  if (q_row_stride < static_cast<int64_t>(q_heads) * head_dim)
+    return fail(B200MOE_ERR_SHAPE, "%s: query row stride %lld smaller than a row", name, (long long)q_row_stride);
+  if (batch == 0) return B200MOE_OK;
+  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !out || !block_table || !context_lens)
+    return fail(B200MOE_ERR_NULL, "%s: null pointer", name);
+  if (!aligned_to(q, 16) || q_row_stride % 8 != 0 || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16))
+    return fail(B200MOE_ERR_ALIGN, "%s: q, its row stride and the caches must be 16-byte aligned", name);
+  if (static_cast<int64_t>(batch) * kv_heads * num_splits > 0x7fffffffLL ||
+      static_cast<int64_t>(batch) * q_heads > 0x7fffffffLL)
+    return fail(B200MOE_ERR_SHAPE, "%s: too many CTAs", name);
+  Params p;
+  p.q = q; p.out = out; p.q_stride = q_row_stride;
+  p.k_cache = static_cast<const uint8_t*>(k_cache); p.v_cache = static_cast<const uint8_t*>(v_cache);
+  p.k_scale = k_scale; p.v_scale = v_scale;
+  p.block_table = block_table; p.context_lens = context_lens; p.table_stride = table_row_stride;
+  p.ws_o = nullptr; p.ws_ml = nullptr;
+  p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = group; p.block_size = block_size;
+  p.max_blocks = max_blocks_per_seq; p.num_splits = num_splits; p.num_blocks = num_blocks;
+  p.scale_log2 = softmax_scale * kLog2e;
+  if (num_splits > 1) {
+    const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits);
+    if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
+      return fail(B200MOE_ERR_WORKSPACE, "%s: num_splits=%d needs a 16-byte aligned workspace of "
+                  "%zu bytes, got %zu", name, num_splits, need, workspace_bytes);
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + static_cast<size_t>(batch) * q_heads * num_splits * kDim;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == B200MOE_BF16)
+    return group <= 8 ? launch<__nv_bfloat16, 1>(p, batch, st) : launch<__nv_bfloat16, 2>(p, batch, st);
+  return group <= 8 ? launch<__half, 1>(p, batch, st) : launch<__half, 2>(p, batch, st);
+}

@@ -394,6 +394,75 @@ int b200moe_paged_attn_varlen(const void* q, const void* k_cache, const void* v_
                               size_t workspace_bytes, b200moe_stream_t stream);
 
 /*
+ * Tables of one serving step, built on the GPU from the requests' lengths.  Replaces the host loops
+ * that fill block tables, slot mapping and positions before every step of the reference's engine
+ * (engine/block_manager.py, engine/model_runner.py).
+ *
+ *   context_lens  i32 [num_requests] tokens of each request in the cache (clamped to what a table row
+ *                 can name)
+ *   new_lens      i32 [num_requests] token rows of this step; 0 waits, negative: the request has ended
+ *   block_table   i32 [num_requests, max_blocks_per_seq], rows table_row_stride elements apart; the
+ *                 entries of newly taken pages are written
+ *   free_blocks   i32 [free_capacity] stack of free pages, the first *free_count entries are in use;
+ *                 the pages of ended requests are pushed, in request order, before any is popped
+ *   seq_lens      i32 [num_requests] lengths after the step (may be context_lens); 0 for ended requests
+ *   cu_seqlens    i32 [num_requests + 1] first token row of each request, at most num_rows
+ *   slot_mapping  i32 [num_rows] cache slot of each row; -1 for rows without one
+ *   positions     optional i64 [num_rows] position of each row in its request; 0 behind the last one
+ *   free_count_out, num_refused  i32 [1] each (free_count_out may be free_count)
+ *
+ * Requests pop the pages they lack from the top of the stack in request order.  A request is refused
+ * (length kept, slots -1, counted in num_refused) when its pages do not fit the table row, when its
+ * rows do not fit num_rows, or when it needs pages and its need together with that of all requests
+ * before it exceeds the free pages.  num_requests <= b200moe_paged_schedule_max_requests() (8192).
+ * One launch; nothing but the two named pairs may overlap.
+ */
+int b200moe_paged_schedule_max_requests(void);
+int b200moe_paged_schedule(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_table,
+                           int32_t* free_blocks, const int32_t* free_count, int64_t num_requests,
+                           int64_t max_blocks_per_seq, int64_t table_row_stride, int block_size,
+                           int64_t free_capacity, int64_t num_rows, int32_t* seq_lens,
+                           int32_t* cu_seqlens, int32_t* slot_mapping, int64_t* positions,
+                           int32_t* free_count_out, int32_t* num_refused, b200moe_stream_t stream);
+
+/*
+ * Paged KV cache in 8 bits (no counterpart in the reference, whose caches hold the model's element
+ * type): e4m3 codes [num_blocks, block_size, num_kv_heads, 128] and one fp32 scale per page and head,
+ * [num_blocks, num_kv_heads], value = code * scale.  Scales are powers of two in [2^-32, 2^32]; one
+ * that is smaller, 0 or NaN (a page that was never stored to) counts as 2^-32.
+ *
+ * b200moe_paged_store_kvcache_fp8 stores token i's key and value rows (any of the three float types;
+ * 16-byte aligned, row strides in elements and multiples of 16 bytes) to slot slot_mapping[i]; negative
+ * slots and slots >= num_blocks * block_size are skipped.  Per page and head that the call stores to:
+ *   scale <- max(old scale, smallest 2^e with |x| <= 448 * 2^e for every finite x of the call)
+ *   when it grew, the page's old codes <- e4m3(code * old scale / scale)
+ *   new codes <- e4m3(x / scale), round to nearest even; NaN stays NaN, infinities become +-448
+ * A call that stores to a page's first slot begins the page anew: its old scale and codes count for
+ * nothing.  Slots must be distinct, and the tokens of one page must follow one another in the call with
+ * nothing but skipped entries between them.  head_dim must be 128.
+ *
+ * b200moe_paged_attn_varlen_fp8 is b200moe_paged_attn_varlen over such caches; q rows are q_row_stride
+ * elements apart (a multiple of 8), table rows table_row_stride.  Scores, softmax statistics and sums
+ * are fp32, the probabilities are rounded to fp16 for the product with V.  A NaN in a context gives NaN;
+ * codes past a context may be anything.
+ */
+int b200moe_paged_store_kvcache_fp8(const void* key, const void* value, void* k_cache, void* v_cache,
+                                    float* k_scale, float* v_scale, const int32_t* slot_mapping,
+                                    int dtype, int64_t num_tokens, int num_kv_heads, int head_dim,
+                                    int64_t key_row_stride, int64_t value_row_stride,
+                                    int64_t num_blocks, int block_size, b200moe_stream_t stream);
+int b200moe_paged_attn_fp8_num_splits(int batch, int kv_heads, int64_t max_context);
+size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int num_splits);
+int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache, const void* v_cache,
+                                  const float* k_scale, const float* v_scale, void* out,
+                                  const int32_t* block_table, const int32_t* context_lens, int dtype,
+                                  int batch, int q_heads, int kv_heads, int head_dim,
+                                  int64_t q_row_stride, int64_t num_blocks, int block_size,
+                                  int max_blocks_per_seq, int64_t table_row_stride,
+                                  float softmax_scale, int num_splits, void* workspace,
+                                  size_t workspace_bytes, b200moe_stream_t stream);
+
+/*
  * The whole layer in one call: router (softmax, top-2, optional renormalisation) -> token alignment
  * with block 128 (writes its own padding) -> gather of the routed rows -> grouped GEMM w13 + SwiGLU
  * -> grouped GEMM w2 x routing weight -> combine, issued back to back on `stream` by the entry
