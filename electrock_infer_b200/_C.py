@@ -549,3 +549,45 @@ def paged_attn_varlen_fp8(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch
     _lib.check(rc, name)
     _lib.count_launches(2 if num_splits > 1 else 1)
     return out
+
+
+def few_tokens_max() -> int:
+    """Most tokens that one ``moe_few_tokens`` call takes."""
+    return _lib.load().b200moe_few_tokens_max()
+
+
+def moe_few_tokens(output: torch.Tensor, hidden_states: torch.Tensor, gating_output: torch.Tensor,
+                   w13: torch.Tensor, w2: torch.Tensor, renormalize: bool = True) -> None:
+    """The whole layer of ``fused_experts`` for 1 to 32 tokens in two kernels that read the weights of
+    the chosen experts once (the reference has one path for all sizes, layers/moe/fused_moe.py:170-293).
+
+    ``hidden_states`` and ``output`` bf16 ``[T, H]`` (may be the same tensor), ``gating_output`` router
+    logits ``[T, 8]`` in any float dtype, ``w13`` bf16 ``[8, 2 * I, H]`` (gate rows first), ``w2`` bf16
+    ``[8, H, I]``; ``H`` a multiple of 16, ``I`` of 8.  Top-2 with the lower index on equal logits.  Unlike
+    ``fused_experts``, which rounds the activations and each expert's rows to bf16 as the reference does, only
+    the result is rounded.  The scratch (``8 * T * I`` bytes) is allocated per call from torch's allocator.
+    """
+    name = "moe_few_tokens"
+    dev = _require_cuda(name, output, hidden_states, gating_output, w13, w2)
+    bf16 = torch.bfloat16
+    if output.dtype != bf16 or hidden_states.dtype != bf16 or w13.dtype != bf16 or w2.dtype != bf16:
+        raise RuntimeError(f"{name}: output, hidden_states, w13 and w2 must be bfloat16")
+    if hidden_states.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+        raise RuntimeError(f"{name}: expected hidden_states [T, H], w13 [E, 2 * I, H] and w2 [E, H, I]")
+    num_tokens, hidden = hidden_states.shape
+    num_experts, inter = w13.size(0), w2.size(2)
+    if (output.shape != hidden_states.shape or gating_output.shape != (num_tokens, num_experts)
+            or w13.shape != (num_experts, 2 * inter, hidden) or w2.shape != (num_experts, hidden, inter)):
+        raise RuntimeError(f"{name}: shapes do not match: output {tuple(output.shape)}, hidden_states "
+                           f"{tuple(hidden_states.shape)}, gating_output {tuple(gating_output.shape)}, "
+                           f"w13 {tuple(w13.shape)}, w2 {tuple(w2.shape)}")
+    tag = _float_tag(name, gating_output)
+    lib = _lib.load()
+    ws_bytes = lib.b200moe_few_tokens_workspace_bytes(num_tokens, inter)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = _call(dev, lib.b200moe_few_tokens,
+               hidden_states.data_ptr(), gating_output.data_ptr(), tag, w13.data_ptr(), w2.data_ptr(),
+               output.data_ptr(), num_tokens, num_experts, 2, hidden, inter, int(renormalize),
+               ws.data_ptr(), ws_bytes)
+    _lib.check(rc, name)
+    _lib.count_launches(2 if num_tokens else 0)

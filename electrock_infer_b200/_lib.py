@@ -80,6 +80,10 @@ SIGNATURES = {
     "b200moe_paged_schedule": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                        c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p, c_void_p]),
+    "b200moe_few_tokens_max": (c_int, []),
+    "b200moe_few_tokens_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "b200moe_few_tokens": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                   c_int, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "b200moe_peer_alloc": (c_int, [c_size_t, ctypes.POINTER(c_void_p), c_void_p]),
     "b200moe_peer_open": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "b200moe_peer_close": (c_int, [c_void_p]),

@@ -220,7 +220,8 @@ def _bf16_weights(w: torch.Tensor) -> torch.Tensor:
 def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
                   gating_output: Optional[torch.Tensor], topk: int, renormalize: bool = True,
                   inplace: bool = False, activation: str = "silu",
-                  gate_weight: Optional[torch.Tensor] = None, tp_reduce=None) -> torch.Tensor:
+                  gate_weight: Optional[torch.Tensor] = None, tp_reduce=None,
+                  few_tokens: bool = False) -> torch.Tensor:
     """Mixture-of-experts forward for ``hidden_states [T, H]`` (reference fused_moe.py:170-293).
 
     ``w1`` is the stacked gate/up weight ``[E, 2*I, H]`` (gate rows first), ``w2`` is
@@ -239,7 +240,10 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
     kernel itself and ``gating_output`` may be ``None``.  With ``tp_reduce`` (a
     ``parallel.TensorParallelReduce`` whose ``usable(num_tokens)`` holds on every rank) the result
     is also summed over the tensor-parallel ranks: the second GEMM stores its rows into the owning
-    ranks' buffers over NVLink and the combine kernel finishes the all-reduce.
+    ranks' buffers over NVLink and the combine kernel finishes the all-reduce.  With ``few_tokens``
+    a batch of at most ``_C.few_tokens_max()`` tokens runs as two kernels that read each chosen
+    expert's weights once (``_C.moe_few_tokens``); it needs ``gating_output``, 8 experts and top-2, and
+    rounds only the result, so its results differ from the general path's in the last bits.
     """
     if activation != "silu":
         raise NotImplementedError(f"Activation {activation} not supported.")
@@ -254,7 +258,7 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
     if hidden_states.dtype != torch.bfloat16:
         # Compute in bf16 like the reference, hand the result back in the caller's dtype.
         result = fused_experts(hidden_states.to(torch.bfloat16), w1, w2, gating_output, topk,
-                               renormalize, True, activation, gate_weight, tp_reduce)
+                               renormalize, True, activation, gate_weight, tp_reduce, few_tokens)
         if inplace:
             return hidden_states.copy_(result)
         return result.to(hidden_states.dtype)
@@ -275,6 +279,13 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
 
     output = hidden_states if inplace else torch.empty_like(hidden_states)
     if num_tokens == 0:
+        return output
+
+    if few_tokens:
+        if gate_weight is not None or tp_reduce is not None or topk != 2:
+            raise RuntimeError("fused_experts: few_tokens needs gating_output, top_k=2 and no tp_reduce")
+        with _timed("moe_few_tokens"):
+            _C.moe_few_tokens(output, hidden_states, gating_output.contiguous(), w1, w2, renormalize=renormalize)
         return output
 
     dev = hidden_states.device

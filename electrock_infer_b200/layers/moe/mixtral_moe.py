@@ -28,6 +28,10 @@ class FusedMoE(nn.Module):
     NVLink peer mappings (``parallel.TensorParallelReduce``; needs ``T`` divisible by ``tp_size``
     and all ranks on one node).  ``"auto"`` (default) uses the peer path when it applies and the
     result is at least ``PEER_REDUCE_MIN_BYTES`` large, else NCCL.
+
+    Extension: batches of up to ``few_token_limit`` tokens (0 to 32; default 0: none) take the two-kernel
+    path ``fused_experts(few_tokens=True)``, whose results differ from the general path's in the last
+    bits.  Needs 8 experts and top-2; a sum over ranks is then NCCL's.
     """
 
     PEER_REDUCE_MIN_BYTES = 4 << 20
@@ -35,8 +39,13 @@ class FusedMoE(nn.Module):
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
                  tp_size: Optional[int] = None, params_dtype: Optional[torch.dtype] = None,
                  renormalize: bool = True, reduce_results: bool = False,
-                 tp_exchange: str = "auto"):
+                 tp_exchange: str = "auto", few_token_limit: int = 0):
         super().__init__()
+        if not 0 <= few_token_limit <= 32:
+            raise ValueError("few_token_limit must lie in 0..32")
+        if few_token_limit and (num_experts != 8 or top_k != 2):
+            raise ValueError("few_token_limit needs 8 experts and top_k=2")
+        self.few_token_limit = few_token_limit
         if tp_exchange not in ("auto", "peer", "nccl"):
             raise ValueError("tp_exchange must be 'auto', 'peer' or 'nccl'")
         self.tp_exchange = tp_exchange
@@ -76,6 +85,8 @@ class FusedMoE(nn.Module):
         if not (self.reduce_results and self.tp_size > 1) or self.tp_exchange == "nccl":
             return None
         num_tokens, hidden = hidden_states.shape
+        if num_tokens <= self.few_token_limit:
+            return None
         applies = (hidden_states.is_cuda and self.top_k == 2 and self.tp_size <= 8
                    and self.tp_size == dist.get_world_size() and dist.get_backend() == "nccl"
                    and num_tokens > 0 and num_tokens % self.tp_size == 0)
@@ -105,7 +116,8 @@ class FusedMoE(nn.Module):
         final_hidden_states = fused_experts(
             hidden_states=hidden_states, w1=self.w13_weight, w2=self.w2_weight,
             gating_output=router_logits, topk=self.top_k, renormalize=self.renormalize,
-            inplace=True, activation="silu", tp_reduce=tp_reduce)
+            inplace=True, activation="silu", tp_reduce=tp_reduce,
+            few_tokens=hidden_states.size(0) <= self.few_token_limit)
         if self.reduce_results and self.tp_size > 1 and tp_reduce is None:
             with _timed("all_reduce:result"):
                 dist.all_reduce(final_hidden_states)
@@ -141,12 +153,14 @@ class MixtralMoE(nn.Module):
     ``forward(hidden_states)`` accepts 1-D or 2-D token shapes, overwrites the tokens with the
     layer output and returns them in the original shape, like the reference.  Unlike the
     reference, the gate projection is not a separate GEMM: the router kernel computes it while it
-    reads the tokens.  ``fuse_gate=False`` restores the separate ``F.linear``.
+    reads the tokens.  ``fuse_gate=False`` restores the separate ``F.linear``, which batches of up to
+    ``few_token_limit`` tokens take too.
     """
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
                  params_dtype: Optional[torch.dtype] = None, tp_size: Optional[int] = None,
-                 prefix: str = "", fuse_gate: bool = True, tp_exchange: str = "auto"):
+                 prefix: str = "", fuse_gate: bool = True, tp_exchange: str = "auto",
+                 few_token_limit: int = 0):
         super().__init__()
         self.hidden_size = hidden_size
         self.fuse_gate = fuse_gate
@@ -157,7 +171,7 @@ class MixtralMoE(nn.Module):
         self.experts = FusedMoE(num_experts=num_experts, top_k=top_k, hidden_size=hidden_size,
                                 intermediate_size=intermediate_size, params_dtype=params_dtype,
                                 reduce_results=True, renormalize=True, tp_size=tp_size,
-                                tp_exchange=tp_exchange)
+                                tp_exchange=tp_exchange, few_token_limit=few_token_limit)
 
     @staticmethod
     def _gate_weight_loader(param: nn.Parameter, loaded_weight: torch.Tensor) -> None:
@@ -167,7 +181,7 @@ class MixtralMoE(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         orig_shape = hidden_states.shape
         hidden_states = hidden_states.view(-1, self.hidden_size)
-        if self.fuse_gate:
+        if self.fuse_gate and hidden_states.size(0) > self.experts.few_token_limit:
             tp_reduce = self.experts.peer_reduce_for(hidden_states)
             out = fused_experts(hidden_states, self.experts.w13_weight, self.experts.w2_weight, None,
                                 self.experts.top_k, renormalize=True, inplace=True,

@@ -491,6 +491,25 @@ int b200moe_fused_experts(const void* hidden_states, const void* gating_output, 
                           b200moe_stream_t stream);
 
 /*
+ * The same layer for 0 to b200moe_few_tokens_max() (32) tokens, in two kernels that read the weights of
+ * the experts that were hit once: bound by HBM at 6 * hidden * inter bytes per expert.  Router (softmax,
+ * top-2, the lower index on equal logits, optional renormalisation) included.  Only the output is rounded to
+ * bf16: the activations between the kernels keep 16 bits of mantissa and all sums are fp32, while
+ * b200moe_fused_experts rounds the activations and every pair's row like the reference.
+ *
+ *   arguments as in b200moe_fused_experts; hidden % 16 == 0, inter % 8 == 0, both at most 2^20;
+ *   output may be hidden_states
+ *   workspace  b200moe_few_tokens_workspace_bytes(num_tokens, inter) bytes, 16-byte aligned; need not be
+ *              initialised; must not be shared by calls that may overlap
+ */
+int b200moe_few_tokens_max(void);
+size_t b200moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t inter);
+int b200moe_few_tokens(const void* hidden_states, const void* gating_output, int logits_dtype,
+                       const void* w13, const void* w2, void* output, int64_t num_tokens,
+                       int num_experts, int top_k, int64_t hidden, int64_t inter, int renormalize,
+                       void* workspace, size_t workspace_bytes, b200moe_stream_t stream);
+
+/*
  * Device-side status word of the grouped GEMMs.  Their waits on memory barriers are bounded; a
  * wait that runs out records a non-zero code here and the kernel returns.  Reading synchronises
  * with the device.  Returns the code (0 = no error) or a negative B200MOE_ERR_*; `reset` != 0

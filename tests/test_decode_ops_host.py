@@ -93,3 +93,32 @@ def test_oracle_codes_agree_with_torch():
     ties = torch.from_numpy((codes[1:] + codes[:-1]) / 2).float()
     assert np.array_equal(decode_oracle.to_code_values(ties.double().numpy()), ties.to(torch.float8_e4m3fn).double().numpy())
     assert decode_oracle.scale_ref(448.0) == 1.0 and decode_oracle.scale_ref(448.5) == 2.0 and decode_oracle.scale_ref(0.0) == 2.0 ** -32
+
+
+def test_few_token_arguments():
+    lib = _lib.load()
+
+    def call(dtype=_lib.F32, tokens=4, experts=8, topk=2, hidden=256, inter=128, x=PTR, ws=PTR, ws_bytes=1 << 20):
+        return lib.b200moe_few_tokens(x, PTR, dtype, PTR, PTR, PTR, tokens, experts, topk, hidden, inter, 1, ws, ws_bytes, None)
+
+    assert lib.b200moe_few_tokens_max() == 32
+    for bad in (dict(tokens=33), dict(tokens=-1), dict(experts=7), dict(topk=1), dict(hidden=250), dict(hidden=0), dict(inter=100),
+                dict(inter=0), dict(hidden=(1 << 20) + 16), dict(inter=(1 << 20) + 8)):
+        assert call(**bad) == -1, bad
+    assert call(dtype=7) == -2 and call(x=None) == -3 and call(x=ctypes.c_void_p(264)) == -5
+    need = lib.b200moe_few_tokens_workspace_bytes(4, 128)
+    assert need == 4 * 2 * 128 * 4 and call(ws_bytes=need - 1) == -4 and call(ws=None) == -4
+    assert call(tokens=0) == 0
+
+
+def test_few_token_layer_arguments():
+    from electrock_infer_b200.layers.moe import FusedMoE, fused_experts
+    for bad in (dict(few_token_limit=33), dict(few_token_limit=-1)):
+        with pytest.raises(ValueError):
+            FusedMoE(8, 2, 64, 256, tp_size=1, **bad)
+    with pytest.raises(ValueError):
+        FusedMoE(4, 2, 64, 256, tp_size=1, few_token_limit=4)
+    assert FusedMoE(8, 2, 64, 256, tp_size=1).few_token_limit == 0
+    with pytest.raises(RuntimeError, match="CUDA"):
+        fused_experts(torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(8, 512, 256, dtype=torch.bfloat16),
+                      torch.zeros(8, 256, 256, dtype=torch.bfloat16), torch.zeros(4, 8), 2, few_tokens=True)
