@@ -29,10 +29,12 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// Two codes in the low 16 bits -> two fp16 values (exact).
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+// Four codes -> fp16 pairs of the two in the low and the two in the high half (exact).  Written as one
+// block so that the halves of the word are register halves and not masks and shifts.
+__device__ __forceinline__ void codes_to_half2(uint32_t codes, uint32_t& low, uint32_t& high) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(low), "=r"(high)
+      : "r"(codes));
 }
 
 // Two fp32 values -> two codes, round to nearest even, too large values to the largest code.
@@ -42,7 +44,8 @@ __device__ __forceinline__ uint32_t to_codes2(float lo, float hi) {
 
 // Four codes multiplied by `ratio` and rounded again.
 __device__ __forceinline__ uint32_t rescale_codes4(uint32_t codes, float ratio) {
-  const uint32_t a = codes_to_half2(codes & 0xffffu), b = codes_to_half2(codes >> 16);
+  uint32_t a, b;
+  codes_to_half2(codes, a, b);
   const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
   const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
   return to_codes2(fa.x * ratio, fa.y * ratio) | (to_codes2(fb.x * ratio, fb.y * ratio) << 16);

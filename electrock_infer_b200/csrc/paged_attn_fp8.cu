@@ -48,7 +48,9 @@ constexpr int kRingBytes = kWarps * kStages * kStageBytes;                    //
 constexpr int kScaleBytes = kWarps * kStages * 2 * kChunkTiles * sizeof(float);
 constexpr int kSmemBytes = kRingBytes + kScaleBytes;                          // two CTAs per SM
 constexpr int kMaxGroup = 16;
+constexpr int kMaxSplits = 64;
 constexpr int kMaxContext = 0x7fffffff - 2 * kChunk;  // so that rounding up to chunks stays in range
+constexpr float kSlack = 8.f;              // in powers of two
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -64,8 +66,16 @@ struct Params {
   float* ws_ml;  // [batch, q_heads, splits, 2] running max (log2 domain) and sum
   int64_t q_stride, num_blocks, table_stride;
   int q_heads, kv_heads, group, block_size, max_blocks, num_splits;
+  uint32_t div_mul, div_shift;  // n / block_size == (n * div_mul) >> 32 >> div_shift for 0 <= n < 2^31
   float scale_log2;
 };
+
+// 2^x with results below 2^-126 flushed to zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Byte offset of 16-byte column `col` of token row `row` in a swizzled tile of 128-byte rows.
 __device__ __forceinline__ uint32_t tile_offset(int row, int col) {
@@ -99,6 +109,13 @@ paged_attn_fp8_kernel(const Params p) {
   const int32_t* table = p.block_table + seq * p.table_stride;
   const int64_t row_bytes = static_cast<int64_t>(p.kv_heads) * kDim;
 
+  // What a lane copies of every tile: column `col` of rows `row`, row + 4, row + 8, row + 12.
+  const int row = lane >> 3, col = lane & 7;
+  const uint32_t dst_even = ring + tile_offset(row, col), dst_odd = ring + tile_offset(row + 4, col);
+  const int64_t row_at = row * row_bytes + kvh * kDim + col * 16;
+  const int64_t v_minus_k = p.v_cache - p.k_cache;
+  const int64_t four_rows = 4 * row_bytes;
+
   // Issues the copies of the CTA's chunk `ci` into ring slot `stage`.  A page outside the cache is
   // replaced by page 0, tokens past the range are filled with zeros (0 * NaN would poison the output).
   auto issue = [&](int ci, int stage) {
@@ -108,21 +125,29 @@ paged_attn_fp8_kernel(const Params p) {
         const int tok = t_begin + ci * kChunk + tile * kTile;
         int page = 0, off = 0;
         if (tok < t_end) {
-          page = table[tok / p.block_size];
-          off = tok % p.block_size;
+          const int index = static_cast<int>(__umulhi(static_cast<uint32_t>(tok), p.div_mul) >> p.div_shift);
+          page = table[index];
+          off = tok - index * p.block_size;
           if (page < 0 || page >= p.num_blocks) page = 0;
         }
-        const int row = lane >> 3, col = lane & 7;
-        const int64_t at = (static_cast<int64_t>(page) * p.block_size + off + (tok < t_end ? row : 0)) * row_bytes +
-                           kvh * kDim + col * 16;
-        const uint32_t dst = ring + stage * kStageBytes + tile * kTile * kDim;
+        const uint8_t* k = p.k_cache + (static_cast<int64_t>(page) * p.block_size + off) * row_bytes + row_at;
+        const uint32_t to = stage * kStageBytes + tile * kTile * kDim;
+        if (tok + kTile <= t_end) {
 #pragma unroll
-        for (int j = 0; j < kTile / 4; ++j) {
-          const int bytes = tok + row + j * 4 < t_end ? 16 : 0;
-          const int64_t from = at + (bytes ? j * 4 * row_bytes : 0);
-          const uint32_t to = dst + tile_offset(row + j * 4, col);
-          cp_async_16(to, p.k_cache + from, bytes);
-          cp_async_16(to + kHalfBytes, p.v_cache + from, bytes);
+          for (int j = 0; j < kTile / 4; ++j, k += four_rows) {
+            const uint32_t dst = (j & 1 ? dst_odd : dst_even) + to + (j & ~1) * 4 * kDim;
+            cp_async_16(dst, k, 16);
+            cp_async_16(dst + kHalfBytes, k + v_minus_k, 16);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kTile / 4; ++j) {
+            const int bytes = tok + row + j * 4 < t_end ? 16 : 0;
+            const uint8_t* from = bytes ? k + j * four_rows : p.k_cache;
+            const uint32_t dst = (j & 1 ? dst_odd : dst_even) + to + (j & ~1) * 4 * kDim;
+            cp_async_16(dst, from, bytes);
+            cp_async_16(dst + kHalfBytes, from + v_minus_k, bytes);
+          }
         }
         if (lane < 2) {
           const float* s = (lane ? p.v_scale : p.k_scale) + static_cast<int64_t>(page) * p.kv_heads + kvh;
@@ -220,58 +245,73 @@ paged_attn_fp8_kernel(const Params p) {
         const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t a[4] = {codes_to_half2(wl[w] & 0xffffu), codes_to_half2(wh[w] & 0xffffu),
-                                 codes_to_half2(wl[w] >> 16), codes_to_half2(wh[w] >> 16)};
+          uint32_t a[4];
+          codes_to_half2(wl[w], a[0], a[2]);
+          codes_to_half2(wh[w], a[1], a[3]);
 #pragma unroll
           for (int n = 0; n < kNT; ++n) Mma<__half>::run(s[tile][n], a, qb[n][h * 4 + w][0], qb[n][h * 4 + w][1]);
         }
       }
-      // Into the exp2 domain; tokens past the range do not count.
+      // Into the exp2 domain.
       const float ks = usable_scale(sc[tile * 2]);
-      const bool v0 = tok0 + tile * kTile + g < t_end, v1 = tok0 + tile * kTile + g + 8 < t_end;
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
-        s[tile][n][0] = v0 ? s[tile][n][0] * (qmul[n][0] * ks) : -INFINITY;
-        s[tile][n][1] = v0 ? s[tile][n][1] * (qmul[n][1] * ks) : -INFINITY;
-        s[tile][n][2] = v1 ? s[tile][n][2] * (qmul[n][0] * ks) : -INFINITY;
-        s[tile][n][3] = v1 ? s[tile][n][3] * (qmul[n][1] * ks) : -INFINITY;
+        const float f0 = qmul[n][0] * ks, f1 = qmul[n][1] * ks;
+        s[tile][n][0] *= f0;
+        s[tile][n][1] *= f1;
+        s[tile][n][2] *= f0;
+        s[tile][n][3] *= f1;
       }
     }
-    // A chunk holds at least one token of the range, so the new maxima are finite.
+    if (tok0 + kChunk > t_end) {  // tokens past the range do not count
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (tok0 + tile * kTile + g + (j >> 1) * 8 >= t_end) s[tile][n][j] = -INFINITY;
+    }
+    // A chunk holds at least one token of the range, so its maxima are finite.  The reference point of a
+    // head's exponentials follows the maximum only when that has risen by more than 2^kSlack: until then
+    // P may reach 2^kSlack, which costs no precision, and nothing has to be rescaled.
     uint32_t pb[kChunkTiles][kNT][2];  // P^T as B fragments
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float alpha[2];
+      float top[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = fmaxf(s[0][n][c], s[0][n][c + 2]);
+        top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
 #pragma unroll
-        for (int tile = 1; tile < kChunkTiles; ++tile) top = fmaxf(top, fmaxf(s[tile][n][c], s[tile][n][c + 2]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        top = fmaxf(top, mx[n][c]);
-        alpha[c] = exp2f(mx[n][c] - top);  // exp2(-inf) = 0 on the first chunk
-        mx[n][c] = top;
-        sum[n][c] *= alpha[c];
+        for (int tile = 1; tile < kChunkTiles; ++tile) top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]));
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+      }
+      if (__any_sync(0xffffffffu, top[0] > mx[n][0] + kSlack || top[1] > mx[n][1] + kSlack)) {
+        const float n0 = fmaxf(mx[n][0], top[0]), n1 = fmaxf(mx[n][1], top[1]);
+        const float a0 = exp2_fast(mx[n][0] - n0), a1 = exp2_fast(mx[n][1] - n1);  // 0 on the first chunk
+        mx[n][0] = n0;
+        mx[n][1] = n1;
+        sum[n][0] *= a0;
+        sum[n][1] *= a1;
 #pragma unroll
-        for (int tile = 0; tile < kChunkTiles; ++tile) {
-          s[tile][n][c] = exp2f(s[tile][n][c] - top);
-          s[tile][n][c + 2] = exp2f(s[tile][n][c + 2] - top);
-          sum[n][c] += s[tile][n][c] + s[tile][n][c + 2];
+        for (int m = 0; m < kDim / 16; ++m) {
+          o[n][m][0] *= a0; o[n][m][1] *= a1;
+          o[n][m][2] *= a0; o[n][m][3] *= a1;
         }
       }
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[tile][n][j] = exp2_fast(s[tile][n][j] - mx[n][j & 1]);
+          sum[n][j & 1] += s[tile][n][j];
+        }
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile) {
         pb[tile][n][0] = transpose_8x8(Mma<__half>::pack(s[tile][n][0], s[tile][n][1]));
         pb[tile][n][1] = transpose_8x8(Mma<__half>::pack(s[tile][n][2], s[tile][n][3]));
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int m = 0; m < kDim / 16; ++m) {
-          o[n][m][0] *= alpha[0]; o[n][m][1] *= alpha[1];
-          o[n][m][2] *= alpha[0]; o[n][m][3] *= alpha[1];
-        }
       }
     }
 #pragma unroll
@@ -298,10 +338,11 @@ paged_attn_fp8_kernel(const Params p) {
         // Bytes of two tokens interleaved: each half is one dim's pair.
         const uint32_t lo0 = __byte_perm(w[0][q], w[1][q], 0x5140), lo1 = __byte_perm(w[0][q], w[1][q], 0x7362);
         const uint32_t hi0 = __byte_perm(w[2][q], w[3][q], 0x5140), hi1 = __byte_perm(w[2][q], w[3][q], 0x7362);
-        const uint32_t a0[4] = {codes_to_half2(lo0 & 0xffffu), codes_to_half2(lo0 >> 16),
-                                codes_to_half2(hi0 & 0xffffu), codes_to_half2(hi0 >> 16)};
-        const uint32_t a1[4] = {codes_to_half2(lo1 & 0xffffu), codes_to_half2(lo1 >> 16),
-                                codes_to_half2(hi1 & 0xffffu), codes_to_half2(hi1 >> 16)};
+        uint32_t a0[4], a1[4];
+        codes_to_half2(lo0, a0[0], a0[1]);
+        codes_to_half2(hi0, a0[2], a0[3]);
+        codes_to_half2(lo1, a1[0], a1[1]);
+        codes_to_half2(hi1, a1[2], a1[3]);
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
           Mma<__half>::run(o[n][2 * q], a0, pb[tile][n][0], pb[tile][n][1]);
@@ -368,24 +409,52 @@ paged_attn_fp8_kernel(const Params p) {
   }
 }
 
-// Merges the splits of one (sequence, query head): thread d owns dimension d.
+// Merges the splits of one (sequence, query head): thread d owns dimension d.  The splits' weights are
+// worked out by one lane each, so that the loads of the partial outputs wait for nothing but themselves.
 template <typename T>
 __global__ void __launch_bounds__(kDim)
 paged_attn_fp8_merge_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
                             T* __restrict__ out, int num_splits) {
+  __shared__ float s_weight[kMaxSplits];
+  __shared__ float s_sum;
   pdl_wait();
   pdl_launch_dependents();
   const int64_t head = blockIdx.x;
   const int d = threadIdx.x;
-  float top = -INFINITY;
-  for (int s = 0; s < num_splits; ++s) top = fmaxf(top, ws_ml[(head * num_splits + s) * 2]);
-  float l = 0.f, acc = 0.f;
-  for (int s = 0; s < num_splits; ++s) {
-    const float ls = ws_ml[(head * num_splits + s) * 2 + 1];
-    const float f = ls == 0.f ? 0.f : exp2f(ws_ml[(head * num_splits + s) * 2] - top);
-    l += f * ls;
-    acc += f * ws_o[(head * num_splits + s) * kDim + d];
+  const float2* ml = reinterpret_cast<const float2*>(ws_ml) + head * num_splits;
+  const float* o = ws_o + head * num_splits * kDim + d;
+  if (d < 32) {
+    float2 v[kMaxSplits / 32];
+    float top = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+      v[i] = d + i * 32 < num_splits ? ml[d + i * 32] : make_float2(-INFINITY, 0.f);
+      top = fmaxf(top, v[i].x);
+    }
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+      const float f = v[i].y == 0.f ? 0.f : exp2f(v[i].x - top);
+      s_weight[d + i * 32] = f;
+      l += f * v[i].y;
+    }
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    if (d == 0) s_sum = l;
   }
+  float acc = 0.f;
+  constexpr int kBatch = 16;
+  for (int s0 = 0; s0 < num_splits; s0 += kBatch) {
+    float v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) v[i] = s0 + i < num_splits ? o[(s0 + i) * kDim] : 0.f;
+    if (s0 == 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (s0 + i < num_splits) acc += s_weight[s0 + i] * v[i];
+  }
+  const float l = s_sum;
   out[head * kDim + d] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
 }
 
@@ -406,8 +475,6 @@ int launch(const Params& p, int batch, cudaStream_t st) {
   }
   return B200MOE_OK;
 }
-
-constexpr int kMaxSplits = 64;
 
 }  // namespace
 }  // namespace b200moe
@@ -475,6 +542,12 @@ extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache,
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = group; p.block_size = block_size;
   p.max_blocks = max_blocks_per_seq; p.num_splits = num_splits; p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * kLog2e;
+  // Division by the block size as a multiplication: with 2^(l - 1) < block_size <= 2^l, the rounded-up
+  // quotient 2^(31 + l) / block_size is exact for dividends below 2^31.
+  int l = 0;
+  while ((1ll << l) < block_size) ++l;
+  p.div_mul = static_cast<uint32_t>(((1ull << (31 + l)) + block_size - 1) / block_size);
+  p.div_shift = static_cast<uint32_t>(l - 1);
   if (num_splits > 1) {
     const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits);
     if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
