@@ -3,13 +3,17 @@
 The ops keep the reference's names, keyword names, output convention (the MoE ops write into
 caller-allocated tensors and return ``None``; ``paged_attn_varlen`` returns a new tensor, as in the
 reference) and error type (``RuntimeError``, what a failed ``TORCH_CHECK`` surfaces as).  Each forwards raw device pointers to the C-ABI
-library on the current CUDA stream of the tensor's device; nothing is computed in Python.
+library on the current CUDA stream of the tensor's device; nothing is computed in Python.  The ops of a
+decode step, whose kernels take microseconds, do so in a compiled binding (csrc/torch_binding.cpp), the
+others through ctypes.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
+
+_binding = None
 
 _FLOAT_TAGS = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _INT_TAGS = {torch.int32: _lib.I32, torch.int64: _lib.I64, torch.int16: _lib.I16,
@@ -33,13 +37,18 @@ def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-def _call(dev: torch.device, fn, *args) -> int:
-    """``fn(*args, stream)`` on the current stream of ``dev``, with ``dev`` current.  Decode-step ops
-    take microseconds on the device, so the guard is entered only when another device is current."""
-    if dev.index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    with torch.cuda.device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _native():
+    """The compiled binding of the decode-step ops (csrc/torch_binding.cpp)."""
+    global _binding
+    if _binding is None:
+        _lib.load()
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise RuntimeError(f"the compiled binding is missing or does not fit this torch ({e}): build it with "
+                               "`python -m electrock_infer_b200.build`") from None
+        _binding = module
+    return _binding
 
 
 def _float_tag(name: str, t: torch.Tensor) -> int:
@@ -404,49 +413,9 @@ def paged_schedule(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tab
     (may be ``free_count``), ``num_refused`` i32 ``[1]``.  New entries are written into ``block_table`` and
     pushed pages into ``free_blocks``.  Apart from the two pairs named, no tensors may overlap.
     """
-    name = "paged_schedule"
-    tensors = [context_lens, new_lens, free_blocks, free_count, seq_lens, cu_seqlens, slot_mapping,
-               free_count_out, num_refused]
-    dev = _require_cuda(name, *tensors)
-    for t in tensors:
-        if t.dtype != torch.int32:
-            raise RuntimeError(f"{name}: lengths, pages and slots must be int32, got {t.dtype}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev:
-        raise RuntimeError(f"{name}: block_table must be int32 [requests, max_blocks] on {dev}")
-    requests, max_blocks = block_table.shape
-    if max_blocks and block_table.stride(1) != 1:
-        raise RuntimeError(f"{name}: the entries of a block_table row must be contiguous")
-    if (context_lens.numel() != requests or new_lens.numel() != requests
-            or seq_lens.numel() != requests or cu_seqlens.numel() != requests + 1):
-        raise RuntimeError(f"{name}: context_lens, new_lens and seq_lens must hold {requests} elements "
-                           f"and cu_seqlens {requests + 1}")
-    if free_count.numel() != 1 or free_count_out.numel() != 1 or num_refused.numel() != 1:
-        raise RuntimeError(f"{name}: free_count, free_count_out and num_refused hold one element")
-    rows = slot_mapping.numel()
-    if positions is not None and (positions.dtype != torch.int64 or positions.numel() != rows
-                                  or positions.device != dev or not positions.is_contiguous()):
-        raise RuntimeError(f"{name}: positions must be contiguous int64 with one entry per row of slot_mapping")
-    rc = _call(dev, _lib.load().b200moe_paged_schedule,
-               context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-               free_blocks.data_ptr(), free_count.data_ptr(), requests, max_blocks,
-               block_table.stride(0) if requests > 1 else max_blocks, block_size,
-               free_blocks.numel(), rows, seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-               slot_mapping.data_ptr(), positions.data_ptr() if positions is not None else None,
-               free_count_out.data_ptr(), num_refused.data_ptr())
-    _lib.check(rc, name)
-    _lib.count_launches(1)
-
-
-def _check_codes(name: str, K_cache: torch.Tensor, V_cache: torch.Tensor,  # noqa: N803
-                 K_scale: torch.Tensor, V_scale: torch.Tensor) -> None:  # noqa: N803
-    if K_cache.dim() != 4 or V_cache.shape != K_cache.shape:
-        raise RuntimeError(f"{name}: caches must both be [blocks, block_size, kv_heads, head_dim]")
-    if K_cache.dtype != torch.float8_e4m3fn or V_cache.dtype != torch.float8_e4m3fn:
-        raise RuntimeError(f"{name}: caches must be float8_e4m3fn, got {K_cache.dtype} and {V_cache.dtype}")
-    shape = (K_cache.size(0), K_cache.size(2))
-    if (K_scale.dtype != torch.float32 or V_scale.dtype != torch.float32 or K_scale.shape != shape
-            or V_scale.shape != shape):
-        raise RuntimeError(f"{name}: scales must be float32 [blocks, kv_heads] = {list(shape)}")
+    (_binding or _native()).paged_schedule(
+        context_lens, new_lens, block_table, free_blocks, free_count, block_size, seq_lens, cu_seqlens, slot_mapping,
+        positions, free_count_out, num_refused)
 
 
 def paged_store_kvcache_fp8(K: torch.Tensor, V: torch.Tensor, K_cache: torch.Tensor,  # noqa: N803
@@ -469,30 +438,7 @@ def paged_store_kvcache_fp8(K: torch.Tensor, V: torch.Tensor, K_cache: torch.Ten
     Slots must be distinct, and the tokens of one page must follow one another in the call with nothing
     but skipped entries between them, as in every slot map that is built request by request.
     """
-    name = "paged_store_kvcache_fp8"
-    dev = _require_cuda(name, K_cache, V_cache, K_scale, V_scale, slot_mapping)
-    _check_codes(name, K_cache, V_cache, K_scale, V_scale)
-    num_blocks, block_size, kv_heads, head_dim = K_cache.shape
-    if K.dim() != 3 or V.shape != K.shape or K.size(1) != kv_heads or K.size(2) != head_dim:
-        raise RuntimeError(f"{name}: K and V must both be [tokens, {kv_heads}, {head_dim}]")
-    if K.device != dev or V.device != dev:
-        raise RuntimeError(f"{name}: K and V must be on {dev}, like the caches")
-    if K.dtype != V.dtype:
-        raise RuntimeError(f"{name}: K and V must share a dtype")
-    num_tokens = K.size(0)
-    for t in (K, V):
-        if t.stride(2) != 1 or (kv_heads > 1 and t.stride(1) != head_dim):
-            raise RuntimeError(f"{name}: the heads of a token must be contiguous")
-    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != num_tokens:
-        raise RuntimeError(f"{name}: slot_mapping must be int32 with one entry per token")
-    row = kv_heads * head_dim
-    rc = _call(dev, _lib.load().b200moe_paged_store_kvcache_fp8,
-               K.data_ptr(), V.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), K_scale.data_ptr(),
-               V_scale.data_ptr(), slot_mapping.data_ptr(), _float_tag(name, K), num_tokens, kv_heads,
-               head_dim, K.stride(0) if num_tokens > 1 else row, V.stride(0) if num_tokens > 1 else row,
-               num_blocks, block_size)
-    _lib.check(rc, name)
-    _lib.count_launches(1 if num_tokens else 0)
+    (_binding or _native()).paged_store_kvcache_fp8(K, V, K_cache, V_cache, K_scale, V_scale, slot_mapping)
 
 
 def paged_attn_varlen_fp8(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch.Tensor,  # noqa: N803
@@ -509,46 +455,8 @@ def paged_attn_varlen_fp8(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch
     choose), the number of ranges that a context is cut into.  The scratch of the merge is allocated per
     call from torch's allocator, so that calls on different streams and captured graphs never share it.
     """
-    name = "paged_attn_varlen_fp8"
-    dev = _require_cuda(name, K_cache, V_cache, K_scale, V_scale, context_lens)
-    _check_codes(name, K_cache, V_cache, K_scale, V_scale)
-    num_blocks, block_size, kv_heads, head_dim = K_cache.shape
-    if Q.dim() != 3 or Q.size(2) != head_dim:
-        raise RuntimeError(f"{name}: Q must be [batch, heads, {head_dim}]")
-    batch, q_heads, _ = Q.shape
-    if Q.device != dev or block_table.device != dev:
-        raise RuntimeError(f"{name}: Q and block_table must be on {dev}, like the caches")
-    if Q.stride(2) != 1 or (q_heads > 1 and Q.stride(1) != head_dim):
-        raise RuntimeError(f"{name}: the heads of a query must be contiguous")
-    if context_lens.dtype != torch.int32 or block_table.dtype != torch.int32:
-        raise RuntimeError(f"{name}: context_lens and block_table must be int32")
-    if block_table.dim() != 2 or block_table.size(0) != batch or context_lens.numel() != batch:
-        raise RuntimeError(f"{name}: block_table must be [batch, max_blocks] and context_lens [batch]")
-    max_blocks = block_table.size(1)
-    if max_blocks > 1 and block_table.stride(1) != 1:
-        raise RuntimeError(f"{name}: the entries of a block_table row must be contiguous")
-    tag = _float_tag(name, Q)
-    lib = _lib.load()
-    out = torch.empty((batch, q_heads, head_dim), dtype=Q.dtype, device=dev)
-    if num_splits <= 0:
-        longest = max_blocks * block_size
-        if 0 < max_seqlen_k < longest:
-            longest = max_seqlen_k
-        num_splits = lib.b200moe_paged_attn_fp8_num_splits(batch, kv_heads, longest)
-    ws, ws_ptr, ws_bytes = None, None, 0
-    if num_splits > 1:
-        ws_bytes = lib.b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        ws_ptr = ws.data_ptr()
-    rc = _call(dev, lib.b200moe_paged_attn_varlen_fp8,
-               Q.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), K_scale.data_ptr(),
-               V_scale.data_ptr(), out.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), tag,
-               batch, q_heads, kv_heads, head_dim, Q.stride(0) if batch > 1 else q_heads * head_dim,
-               num_blocks, block_size, max_blocks, block_table.stride(0) if batch > 1 else max_blocks,
-               float(softmax_scale), num_splits, ws_ptr, ws_bytes)
-    _lib.check(rc, name)
-    _lib.count_launches(2 if num_splits > 1 else 1)
-    return out
+    return (_binding or _native()).paged_attn_varlen_fp8(
+        Q, K_cache, V_cache, K_scale, V_scale, max_seqlen_k, context_lens, block_table, softmax_scale, num_splits)
 
 
 def few_tokens_max() -> int:
@@ -567,27 +475,4 @@ def moe_few_tokens(output: torch.Tensor, hidden_states: torch.Tensor, gating_out
     ``fused_experts``, which rounds the activations and each expert's rows to bf16 as the reference does, only
     the result is rounded.  The scratch (``8 * T * I`` bytes) is allocated per call from torch's allocator.
     """
-    name = "moe_few_tokens"
-    dev = _require_cuda(name, output, hidden_states, gating_output, w13, w2)
-    bf16 = torch.bfloat16
-    if output.dtype != bf16 or hidden_states.dtype != bf16 or w13.dtype != bf16 or w2.dtype != bf16:
-        raise RuntimeError(f"{name}: output, hidden_states, w13 and w2 must be bfloat16")
-    if hidden_states.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
-        raise RuntimeError(f"{name}: expected hidden_states [T, H], w13 [E, 2 * I, H] and w2 [E, H, I]")
-    num_tokens, hidden = hidden_states.shape
-    num_experts, inter = w13.size(0), w2.size(2)
-    if (output.shape != hidden_states.shape or gating_output.shape != (num_tokens, num_experts)
-            or w13.shape != (num_experts, 2 * inter, hidden) or w2.shape != (num_experts, hidden, inter)):
-        raise RuntimeError(f"{name}: shapes do not match: output {tuple(output.shape)}, hidden_states "
-                           f"{tuple(hidden_states.shape)}, gating_output {tuple(gating_output.shape)}, "
-                           f"w13 {tuple(w13.shape)}, w2 {tuple(w2.shape)}")
-    tag = _float_tag(name, gating_output)
-    lib = _lib.load()
-    ws_bytes = lib.b200moe_few_tokens_workspace_bytes(num_tokens, inter)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = _call(dev, lib.b200moe_few_tokens,
-               hidden_states.data_ptr(), gating_output.data_ptr(), tag, w13.data_ptr(), w2.data_ptr(),
-               output.data_ptr(), num_tokens, num_experts, 2, hidden, inter, int(renormalize),
-               ws.data_ptr(), ws_bytes)
-    _lib.check(rc, name)
-    _lib.count_launches(2 if num_tokens else 0)
+    (_binding or _native()).moe_few_tokens(output, hidden_states, gating_output, w13, w2, renormalize)

@@ -1,7 +1,8 @@
-"""Builds libb200moe.so (the C-ABI library, declared in include/b200moe.h) with nvcc for sm_100a.
+"""Builds libb200moe.so (the C-ABI library, declared in include/b200moe.h) with nvcc for sm_100a, and
+_binding.so (csrc/torch_binding.cpp, the decode-step ops for torch tensors) with the host compiler.
 
-Run as ``python -m electrock_infer_b200.build``.  The shared object is written next to this
-file so that it is found by :mod:`electrock_infer_b200._lib` and travels with the source tree.
+Run as ``python -m electrock_infer_b200.build``.  The shared objects are written next to this
+file so that they are found by :mod:`electrock_infer_b200._lib` and travel with the source tree.
 """
 from __future__ import annotations
 
@@ -15,6 +16,8 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libb200moe.so"
 INCLUDE_DIR = PKG_DIR.parent / "include"
+BINDING_PATH = PKG_DIR / "_binding.so"
+BINDING_SOURCE = CSRC / "torch_binding.cpp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -44,9 +47,39 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > built for p in deps)
 
 
+def binding_is_stale() -> bool:
+    if not BINDING_PATH.exists():
+        return True
+    built = BINDING_PATH.stat().st_mtime
+    return any(p.stat().st_mtime > built for p in [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h")])
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compiles the binding against the torch of this interpreter; needs libb200moe.so in place."""
+    if not force and not binding_is_stale():
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    includes = [sysconfig.get_paths()["include"], home / "include", home / "include/torch/csrc/api/include",
+                cuda / "include"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-o", str(BINDING_PATH), str(BINDING_SOURCE), *(f"-I{d}" for d in includes),
+           f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", f"-L{home / 'lib'}",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles every kernel into one shared library; returns its path."""
+    """Compiles every kernel into one shared library, and the binding; returns the library's path."""
     if not force and not is_stale():
+        build_binding()
         return LIB_PATH
     cmd = [find_nvcc(), *NVCC_FLAGS]
     if verbose:
@@ -57,6 +90,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     if verbose:
         print(proc.stderr)
+    build_binding(force)
     return LIB_PATH
 
 
