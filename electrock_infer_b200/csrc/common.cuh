@@ -35,6 +35,22 @@ inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintp
 
 __host__ __device__ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Division of 0 <= n < 2^31 by a positive constant of the launch as a multiplication: with
+// 2^(l - 1) < d <= 2^l the rounded-up quotient 2^(31 + l) / d has 32 bits, and its product with n, shifted
+// back, is exact (the error n / 2^(31 + l) is below 1 / d).
+struct FastDiv {
+  uint32_t mul, shift;  // mul == 0: the divisor is 1
+  static FastDiv by(uint32_t d) {
+    if (d <= 1) return {0, 0};
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    return {static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d), l - 1};
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), mul) >> shift) : n;
+  }
+};
+
 // Programmatic dependent launch.  Every kernel of the layer is launched with the
 // programmatic-stream-serialization attribute: it may begin (block scheduling, prologue) while
 // its predecessor in the stream is still draining, and must call pdl_wait() before it touches

@@ -42,6 +42,7 @@ struct Params {
   const int32_t* slots;
   int64_t num_tokens, num_slots;
   int heads, block_size, segment;
+  FastDiv by_block;
 };
 
 template <typename T> struct Row;   // how a warp holds rows of 128 elements in 16-byte pieces
@@ -84,7 +85,7 @@ __device__ __forceinline__ int32_t slot_of(const Params& p, int64_t i) {
 // Page of token `i`; -1 when the token has no slot.
 __device__ __forceinline__ int page_of(const Params& p, int64_t i) {
   const int32_t s = slot_of(p, i);
-  return s >= 0 ? s / p.block_size : -1;
+  return s >= 0 ? p.by_block(s) : -1;
 }
 
 // Stores the run of `len` tokens from `first`, all in page `page` or skipped, for one head of keys or
@@ -330,6 +331,7 @@ extern "C" int b200moe_paged_store_kvcache_fp8(const void* key, const void* valu
   p.heads = num_kv_heads;
   p.block_size = block_size;
   p.segment = 0;
+  p.by_block = FastDiv::by(static_cast<uint32_t>(block_size));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case B200MOE_BF16: return launch<__nv_bfloat16>(p, st);

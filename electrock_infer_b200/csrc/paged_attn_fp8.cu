@@ -66,7 +66,7 @@ struct Params {
   float* ws_ml;  // [batch, q_heads, splits, 2] running max (log2 domain) and sum
   int64_t q_stride, num_blocks, table_stride;
   int q_heads, kv_heads, group, block_size, max_blocks, num_splits;
-  uint32_t div_mul, div_shift;  // n / block_size == (n * div_mul) >> 32 >> div_shift for 0 <= n < 2^31
+  FastDiv by_block;
   float scale_log2;
 };
 
@@ -125,7 +125,7 @@ paged_attn_fp8_kernel(const Params p) {
         const int tok = t_begin + ci * kChunk + tile * kTile;
         int page = 0, off = 0;
         if (tok < t_end) {
-          const int index = static_cast<int>(__umulhi(static_cast<uint32_t>(tok), p.div_mul) >> p.div_shift);
+          const int index = p.by_block(tok);
           page = table[index];
           off = tok - index * p.block_size;
           if (page < 0 || page >= p.num_blocks) page = 0;
@@ -542,12 +542,7 @@ extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache,
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = group; p.block_size = block_size;
   p.max_blocks = max_blocks_per_seq; p.num_splits = num_splits; p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * kLog2e;
-  // Division by the block size as a multiplication: with 2^(l - 1) < block_size <= 2^l, the rounded-up
-  // quotient 2^(31 + l) / block_size is exact for dividends below 2^31.
-  int l = 0;
-  while ((1ll << l) < block_size) ++l;
-  p.div_mul = static_cast<uint32_t>(((1ull << (31 + l)) + block_size - 1) / block_size);
-  p.div_shift = static_cast<uint32_t>(l - 1);
+  p.by_block = FastDiv::by(static_cast<uint32_t>(block_size));
   if (num_splits > 1) {
     const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits);
     if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))

@@ -11,13 +11,13 @@
 //
 // The reference builds these tables on the host, page by page, and copies them over on every step.
 // Three prefix sums over the requests are all that the rows, pops and pushes have in common, so every
-// CTA of one thread-block cluster computes them for itself in shared memory (a few thousand
-// lengths: 32 KB, cheaper than any exchange), and then the token rows, the popped and the pushed
-// pages are dealt over the cluster's threads, each of which finds its request by bisection of a
-// prefix.  Nothing of what the cluster writes is read again by it (a page popped from
-// the part of the stack that this step pushes is looked up in the releasing request's table row), so
-// the one barrier between the sums and the writes only serves callers that pass the same tensor for
-// lengths before and after.  Bound by latency: a load, three block-wide sums, a bisection, a load and a
+// CTA computes them for itself in shared memory (a few thousand lengths: 32 KB, cheaper than any
+// exchange), and then the token rows, the popped and the pushed
+// pages are dealt over the grid's threads, each of which finds its request by bisection of a
+// prefix.  Prefixes saturate at 2^31 - 1, beyond every limit.  Nothing of what the grid writes is read again by it (a page popped from
+// the part of the stack that this step pushes is looked up in the releasing request's table row), so no
+// barrier is needed, except for callers that pass the same tensor for lengths before and after: their grid
+// is one thread-block cluster of up to eight CTAs with a barrier between the sums and the writes.  Bound by latency: a load, three block-wide sums, a bisection, a load and a
 // store in a chain.
 #include <cooperative_groups.h>
 
@@ -30,8 +30,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxRequests = 8192;
 constexpr int kMaxThreads = 1024;
-constexpr int kMaxPerThread = kMaxRequests / kMaxThreads;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxGrid = 64;
 constexpr int kRowsPerThread = 4;  // consecutive token rows: one 16-byte store of slots
 constexpr int32_t kIntMax = 0x7fffffff;
 
@@ -49,36 +49,49 @@ struct Params {
   int32_t* num_refused;
   int64_t table_stride;
   int32_t requests, max_blocks, block_size, free_capacity, num_rows, vector_rows;
+  FastDiv by_block;
+  int32_t in_place;  // outputs overwrite inputs: the grid is one cluster
 };
 
-__device__ __forceinline__ int32_t saturate(int64_t v) {
-  return v > kIntMax ? kIntMax : static_cast<int32_t>(v);
+// Sum of two non-negative values, at most kIntMax.  Associative, so prefixes may be built in any order; a
+// prefix that reached kIntMax lies beyond every limit it is compared with.
+__device__ __forceinline__ int32_t add_sat(int32_t a, int32_t b) {
+  return static_cast<int32_t>(min(static_cast<uint32_t>(a) + static_cast<uint32_t>(b), static_cast<uint32_t>(kIntMax)));
 }
 
-// Exclusive prefix of `v` over the block; `total` receives the sum.  All threads must call it.
-__device__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_t& total) {
+// Exclusive prefixes of N values over the block (added by add_sat) and their totals, with one barrier.
+// Every warp adds up the warps' sums for itself.  `s_warp` must not be in use by another scan.
+template <int N>
+__device__ __forceinline__ void block_scan(const int32_t (&v)[N], int32_t (*s_warp)[32], int32_t (&before)[N],
+                                           int32_t (&total)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int64_t inc = v;
+  int32_t inc[N];
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
-  }
-  __syncthreads();  // s_warp may still be read from the previous scan
-  if (lane == 31) s_warp[warp] = inc;
+  for (int k = 0; k < N; ++k) inc[k] = v[k];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int32_t o = __shfl_up_sync(0xffffffffu, inc[k], d);
+      if (lane >= d) inc[k] = add_sat(inc[k], o);
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s_warp[k][warp] = inc[k];
   __syncthreads();
-  if (warp == 0) {
-    int64_t w = lane < warps ? s_warp[lane] : 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    int32_t w = lane < warps ? s_warp[k][lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += o;
+      const int32_t o = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w = add_sat(w, o);
     }
-    s_warp[lane] = w;  // inclusive over warps; lanes past the last warp repeat the total
+    total[k] = __shfl_sync(0xffffffffu, w, 31);
+    const int32_t earlier = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    const int32_t own = __shfl_up_sync(0xffffffffu, inc[k], 1);
+    before[k] = add_sat(warp ? earlier : 0, lane ? own : 0);
   }
-  __syncthreads();
-  total = s_warp[31];
-  return inc - v + (warp ? s_warp[warp - 1] : 0);
 }
 
 // First index in [lo, n) with a[index] > key (n if none); `a` does not decrease.
@@ -90,160 +103,190 @@ __device__ __forceinline__ int first_above(const int32_t* a, int lo, int n, int3
   return lo;
 }
 
+// What the blocks know after the sums.
+struct Sums {
+  const int32_t* end;    // rows, inclusive prefix
+  const int32_t* upto;   // pages needed, inclusive prefix
+  const int32_t* rel;    // pages released, inclusive prefix
+  const int32_t* ctx;    // tokens before the step; ~tokens for requests that are not served
+  int32_t top, avail;    // free pages before and after the pushes
+  int requests;
+};
+
+__device__ __forceinline__ int32_t prefix_before(const int32_t* inclusive, int r) { return r ? inclusive[r - 1] : 0; }
+
+// Where page v of the stack, as it stands after the pushes, is to be read.
+__device__ __forceinline__ const int32_t* stack_at(const Params& p, const Sums& s, int32_t v) {
+  if (v < s.top) return p.free_blocks + v;
+  const int r = first_above(s.rel, 0, s.requests, v - s.top);
+  return p.block_table + r * p.table_stride + (v - s.top - prefix_before(s.rel, r));
+}
+
+// Slots and positions of kN consecutive rows from n0.
+template <int kN>
+__device__ __forceinline__ void place_rows(const Params& p, const Sums& s, int64_t n0, int used_rows) {
+  const int32_t* from[kN];  // table or stack entry of the row's page; null: no slot
+  int32_t off[kN];
+  int64_t pos[kN];
+  int r = 0, page_before = -1;
+  int32_t end = 0, start = 0;
+  const int32_t* at = nullptr;
+#pragma unroll
+  for (int u = 0; u < kN; ++u) {
+    const int64_t n = n0 + u;
+    from[u] = nullptr;
+    pos[u] = 0;
+    off[u] = 0;
+    if (n >= used_rows) continue;
+    if (n >= end) {  // u == 0, or the next request begins here
+      r = first_above(s.end, u ? r + 1 : 0, s.requests, static_cast<int32_t>(n));
+      end = s.end[r];
+      start = prefix_before(s.end, r);
+      page_before = -1;
+    }
+    const int32_t c = s.ctx[r];
+    const int32_t base = c < 0 ? ~c : c;
+    pos[u] = static_cast<int64_t>(base) + (n - start);
+    if (c < 0) continue;  // not served: no slot
+    const int32_t i = static_cast<int32_t>(pos[u]);  // served: within the table row
+    const int page = p.by_block(i);
+    if (page != page_before) {
+      page_before = page;
+      const int have = p.by_block(base + p.block_size - 1);
+      at = page < have ? p.block_table + r * p.table_stride + page
+                       : stack_at(p, s, s.avail - 1 - prefix_before(s.upto, r) - (page - have));
+    }
+    from[u] = at;
+    off[u] = i - page * p.block_size;
+  }
+  int32_t page_id[kN], slot[kN];
+#pragma unroll
+  for (int u = 0; u < kN; ++u) page_id[u] = from[u] ? *from[u] : -1;
+#pragma unroll
+  for (int u = 0; u < kN; ++u) {
+    const int64_t at_slot = static_cast<int64_t>(page_id[u]) * p.block_size + off[u];
+    slot[u] = page_id[u] >= 0 && at_slot <= kIntMax ? static_cast<int32_t>(at_slot) : -1;
+  }
+  if (kN == 4 && p.vector_rows && n0 + kN <= p.num_rows) {
+    *reinterpret_cast<int4*>(p.slot_mapping + n0) = make_int4(slot[0], slot[1 % kN], slot[2 % kN], slot[3 % kN]);
+    if (p.positions) {
+      *reinterpret_cast<longlong2*>(p.positions + n0) = make_longlong2(pos[0], pos[1 % kN]);
+      *reinterpret_cast<longlong2*>(p.positions + n0 + 2) = make_longlong2(pos[2 % kN], pos[3 % kN]);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kN; ++u) {
+      if (n0 + u < p.num_rows) {
+        p.slot_mapping[n0 + u] = slot[u];
+        if (p.positions) p.positions[n0 + u] = pos[u];
+      }
+    }
+  }
+}
+
+template <int kPer>  // requests per thread
 __global__ void __launch_bounds__(kMaxThreads)
 paged_schedule_kernel(const Params p) {
   extern __shared__ int32_t smem[];
-  __shared__ int64_t s_warp[32];
+  __shared__ int32_t s_warp[3][32];
   __shared__ int s_refused, s_taken;
   const int R = p.requests, P = p.block_size;
-  int32_t* s_end = smem;          // rows, inclusive prefix
-  int32_t* s_upto = s_end + R;    // pages needed, inclusive prefix
-  int32_t* s_rel = s_upto + R;    // pages released, inclusive prefix
-  int32_t* s_ctx = s_rel + R;     // tokens before the step; ~tokens for requests that are not served
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ncta = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
+  int32_t* s_end = smem;
+  int32_t* s_upto = s_end + R;
+  int32_t* s_rel = s_upto + R;
+  int32_t* s_ctx = s_rel + R;
+  if (threadIdx.x == 0) { s_refused = 0; s_taken = 0; }
   pdl_wait();
   pdl_launch_dependents();
 
-  if (threadIdx.x == 0) { s_refused = 0; s_taken = 0; }
-  const int per = (R + blockDim.x - 1) / blockDim.x;
-  const int i0 = threadIdx.x * per;
-  int32_t rows[kMaxPerThread], ctx[kMaxPerThread];
-  int64_t sum_rows = 0, sum_rel = 0;
+  const int32_t count = *p.free_count;
+  const int i0 = threadIdx.x * kPer;
+  int32_t rows[kPer], ctx[kPer];
+  int32_t sum[2] = {0, 0}, before[2], total[2];  // rows, released pages
 #pragma unroll
-  for (int u = 0; u < kMaxPerThread; ++u) {
-    rows[u] = 0;
-    ctx[u] = 0;
-    if (u < per && i0 + u < R) {
-      ctx[u] = min(max(p.context_lens[i0 + u], 0), p.max_blocks * P);
-      rows[u] = p.new_lens[i0 + u];
-      if (rows[u] > 0) sum_rows += rows[u];
-      else if (rows[u] < 0) sum_rel += (ctx[u] + P - 1) / P;
-    }
+  for (int u = 0; u < kPer; ++u) {
+    const bool live = i0 + u < R;
+    ctx[u] = live ? p.context_lens[i0 + u] : 0;
+    rows[u] = live ? p.new_lens[i0 + u] : 0;
   }
-  int64_t total_rows, total_rel, total_need;
-  int64_t at_rows = block_scan(sum_rows, s_warp, total_rows);
-  int64_t at_rel = block_scan(sum_rel, s_warp, total_rel);
-  const int32_t top = min(max(*p.free_count, 0), p.free_capacity);
-  const int32_t avail = static_cast<int32_t>(min(top + total_rel, static_cast<int64_t>(p.free_capacity)));
-
-  int64_t need[kMaxPerThread], sum_need = 0;
-  bool fits[kMaxPerThread];
 #pragma unroll
-  for (int u = 0; u < kMaxPerThread; ++u) {
+  for (int u = 0; u < kPer; ++u) {
+    ctx[u] = min(max(ctx[u], 0), p.max_blocks * P);
+    if (rows[u] > 0) sum[0] = add_sat(sum[0], rows[u]);
+    else if (rows[u] < 0) sum[1] = add_sat(sum[1], p.by_block(ctx[u] + P - 1));
+  }
+  block_scan<2>(sum, s_warp, before, total);
+  const int32_t top = min(max(count, 0), p.free_capacity);
+  const int32_t avail = min(add_sat(top, total[1]), p.free_capacity);
+
+  int32_t need[kPer], sum_need[1] = {0}, need_before[1], total_need[1];
+  bool fits[kPer];
+  int32_t at_rows = before[0], at_rel = before[1];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
     need[u] = 0;
     fits[u] = false;
-    if (u < per && i0 + u < R) {
-      const int64_t have = (ctx[u] + P - 1) / P;
+    if (i0 + u < R) {
+      const int32_t have = p.by_block(ctx[u] + P - 1);
       if (rows[u] > 0) {
-        at_rows += rows[u];
-        const int64_t want = (static_cast<int64_t>(ctx[u]) + rows[u] + P - 1) / P;
-        fits[u] = want <= p.max_blocks && at_rows <= p.num_rows;
-        if (fits[u]) need[u] = want - have;
+        at_rows = add_sat(at_rows, rows[u]);
+        fits[u] = rows[u] <= p.max_blocks * P - ctx[u] && at_rows <= p.num_rows;
+        if (fits[u]) need[u] = p.by_block(ctx[u] + rows[u] + P - 1) - have;
       } else if (rows[u] < 0) {
-        at_rel += have;
+        at_rel = add_sat(at_rel, have);
       }
-      s_end[i0 + u] = saturate(at_rows);
-      s_rel[i0 + u] = saturate(at_rel);
-      sum_need += need[u];
+      s_end[i0 + u] = at_rows;
+      s_rel[i0 + u] = at_rel;
+      sum_need[0] = add_sat(sum_need[0], need[u]);
     }
   }
-  int64_t at_need = block_scan(sum_need, s_warp, total_need);
+  block_scan<1>(sum_need, s_warp + 2, need_before, total_need);
   int refused = 0, taken = 0;
+  int32_t at_need = need_before[0];
 #pragma unroll
-  for (int u = 0; u < kMaxPerThread; ++u) {
-    if (u < per && i0 + u < R) {
-      at_need += need[u];
+  for (int u = 0; u < kPer; ++u) {
+    if (i0 + u < R) {
+      at_need = add_sat(at_need, need[u]);
       const bool ok = fits[u] && (need[u] == 0 || at_need <= avail);
-      s_upto[i0 + u] = saturate(at_need);
+      s_upto[i0 + u] = at_need;
       s_ctx[i0 + u] = ok ? ctx[u] : ~ctx[u];
       if (rows[u] > 0 && !ok) ++refused;
-      if (ok) taken += static_cast<int>(need[u]);  // the sum over all threads is at most avail
+      if (ok) taken += need[u];  // the sum over all threads is at most avail
     }
   }
   if (refused) atomicAdd(&s_refused, refused);
   if (taken) atomicAdd(&s_taken, taken);
   __syncthreads();
-  // Every CTA holds its own copy of the lengths now: they may be overwritten (seq_lens may be
-  // context_lens, free_count_out may be free_count).
-  if (ncta > 1) cluster.sync();
+  // Every CTA of the cluster holds its own copy of the lengths now: they may be overwritten.
+  if (p.in_place) cg::this_cluster().sync();
 
-  const int first = rank * blockDim.x + threadIdx.x, stride = ncta * blockDim.x;
-  const int used_rows = static_cast<int>(min(total_rows, static_cast<int64_t>(p.num_rows)));
-
-  // Page v of the stack as it stands after the pushes.
-  auto stack = [&](int32_t v) -> int32_t {
-    if (v < top) return p.free_blocks[v];
-    const int r = first_above(s_rel, 0, R, v - top);
-    return p.block_table[r * p.table_stride + (v - top - (r ? s_rel[r - 1] : 0))];
-  };
-
-  // Token rows.
-  for (int64_t n0 = static_cast<int64_t>(first) * kRowsPerThread; n0 < p.num_rows;
-       n0 += static_cast<int64_t>(stride) * kRowsPerThread) {
-    int32_t slot[kRowsPerThread];
-    int64_t pos[kRowsPerThread];
-    int r = 0, last_page = -1;
-    int32_t end = 0, start = 0, page_id = -1;
-#pragma unroll
-    for (int u = 0; u < kRowsPerThread; ++u) {
-      const int64_t n = n0 + u;
-      slot[u] = -1;
-      pos[u] = 0;
-      if (n >= used_rows) continue;
-      if (n >= end) {  // u == 0, or the next request begins here
-        r = first_above(s_end, u ? r + 1 : 0, R, static_cast<int32_t>(n));
-        end = s_end[r];
-        start = r ? s_end[r - 1] : 0;
-        last_page = -1;
-      }
-      const int32_t c = s_ctx[r];
-      const int32_t base = c < 0 ? ~c : c;
-      pos[u] = static_cast<int64_t>(base) + (n - start);
-      if (c < 0) continue;  // not served: no slot
-      const int32_t pi = static_cast<int32_t>(pos[u]);  // served: within the table row
-      const int page = pi / P, have = (base + P - 1) / P;
-      if (page != last_page) {
-        last_page = page;
-        page_id = page < have ? p.block_table[r * p.table_stride + page]
-                              : stack(avail - 1 - (r ? s_upto[r - 1] : 0) - (page - have));
-      }
-      const int64_t s = static_cast<int64_t>(page_id) * P + (pi - page * P);
-      if (page_id >= 0 && s <= kIntMax) slot[u] = static_cast<int32_t>(s);
-    }
-    if (p.vector_rows && n0 + kRowsPerThread <= p.num_rows) {
-      *reinterpret_cast<int4*>(p.slot_mapping + n0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-      if (p.positions) {
-        *reinterpret_cast<longlong2*>(p.positions + n0) = make_longlong2(pos[0], pos[1]);
-        *reinterpret_cast<longlong2*>(p.positions + n0 + 2) = make_longlong2(pos[2], pos[3]);
-      }
+  // The work is dealt over the grid's threads as one sequence: groups of rows, popped pages, pushed
+  // pages, requests.
+  const Sums s = {s_end, s_upto, s_rel, s_ctx, top, avail, R};
+  const int first = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
+  const int used_rows = min(total[0], p.num_rows);
+  const int per_group = p.num_rows > stride ? kRowsPerThread : 1;
+  const int64_t groups = (p.num_rows + per_group - 1) / per_group;
+  const int64_t pops = groups + s_taken, pushes = pops + (avail - top), all = pushes + R;
+  for (int64_t w = first; w < all; w += stride) {
+    if (w < groups) {
+      if (per_group == 1) place_rows<1>(p, s, w, used_rows);
+      else place_rows<kRowsPerThread>(p, s, w * kRowsPerThread, used_rows);
+    } else if (w < pops) {
+      const int k = static_cast<int>(w - groups);
+      const int r = first_above(s_upto, 0, R, k);
+      const int col = p.by_block(s_ctx[r] + P - 1) + (k - prefix_before(s_upto, r));
+      p.block_table[r * p.table_stride + col] = *stack_at(p, s, avail - 1 - k);
+    } else if (w < pushes) {
+      const int v = top + static_cast<int>(w - pops);
+      p.free_blocks[v] = *stack_at(p, s, v);
     } else {
-#pragma unroll
-      for (int u = 0; u < kRowsPerThread; ++u) {
-        if (n0 + u < p.num_rows) {
-          p.slot_mapping[n0 + u] = slot[u];
-          if (p.positions) p.positions[n0 + u] = pos[u];
-        }
-      }
+      const int i = static_cast<int>(w - pushes);
+      const int32_t c = s_ctx[i];
+      const int32_t n = min(s_end[i], p.num_rows), n_prev = min(prefix_before(s_end, i), p.num_rows);
+      p.cu_seqlens[i + 1] = n;
+      p.seq_lens[i] = c >= 0 ? c + (n - n_prev) : s_rel[i] > prefix_before(s_rel, i) ? 0 : ~c;
     }
-  }
-
-  // Popped pages into the table rows, pushed pages onto the stack.
-  for (int k = first; k < s_taken; k += stride) {
-    const int r = first_above(s_upto, 0, R, k);
-    const int col = (s_ctx[r] + P - 1) / P + (k - (r ? s_upto[r - 1] : 0));
-    p.block_table[r * p.table_stride + col] = stack(avail - 1 - k);
-  }
-  for (int v = top + first; v < avail; v += stride) p.free_blocks[v] = stack(v);
-
-  // Lengths and offsets.
-  for (int i = first; i < R; i += stride) {
-    const int32_t c = s_ctx[i];
-    const int32_t n = min(s_end[i], p.num_rows), n_prev = i ? min(s_end[i - 1], p.num_rows) : 0;
-    const int32_t rel = s_rel[i] - (i ? s_rel[i - 1] : 0);
-    p.cu_seqlens[i + 1] = n;
-    p.seq_lens[i] = c >= 0 ? c + (n - n_prev) : rel > 0 ? 0 : ~c;
   }
   if (first == 0) {
     p.cu_seqlens[0] = 0;
@@ -275,7 +318,7 @@ extern "C" int b200moe_paged_schedule(const int32_t* context_lens, const int32_t
     return fail(B200MOE_ERR_SHAPE, "%s: block_size=%d max_blocks_per_seq=%lld row stride %lld (a table "
                 "row must name fewer than 2^31 tokens)", name, block_size,
                 (long long)max_blocks_per_seq, (long long)table_row_stride);
-  if (free_capacity < 0 || free_capacity > kIntMax || num_rows < 0 || num_rows >= kIntMax)
+  if (free_capacity < 0 || free_capacity >= kIntMax || num_rows < 0 || num_rows >= kIntMax)
     return fail(B200MOE_ERR_SHAPE, "%s: free_capacity=%lld num_rows=%lld", name,
                 (long long)free_capacity, (long long)num_rows);
   if (!free_count || !cu_seqlens || !free_count_out || !num_refused || (num_rows > 0 && !slot_mapping) ||
@@ -291,19 +334,29 @@ extern "C" int b200moe_paged_schedule(const int32_t* context_lens, const int32_t
   p.requests = static_cast<int32_t>(num_requests);
   p.max_blocks = static_cast<int32_t>(max_blocks_per_seq);
   p.block_size = block_size;
+  p.by_block = FastDiv::by(static_cast<uint32_t>(block_size));
   p.free_capacity = static_cast<int32_t>(free_capacity);
   p.num_rows = static_cast<int32_t>(num_rows);
   p.vector_rows = aligned_to(slot_mapping, 16) && aligned_to(positions, 16);
 
-  // One CTA of 256 threads for small steps, else 1024 threads and a cluster that grows with the rows.
-  const int threads = num_requests <= 256 && num_rows <= 1024 ? 256 : kMaxThreads;
+  // One CTA of 256 threads for small steps; else 1024 threads and a grid that grows with the work, which is
+  // the rows, the requests and the pages that move (a few per request, the host does not know).
+  p.in_place = seq_lens == context_lens || free_count_out == free_count;
+  const int64_t items = num_rows + 4 * num_requests;
+  const int threads = items <= 512 ? 256 : kMaxThreads;
+  const int most = p.in_place ? kMaxCluster : kMaxGrid;
   int ncta = 1;
-  while (ncta < kMaxCluster && num_rows > static_cast<int64_t>(ncta) * kMaxThreads * kRowsPerThread) ncta *= 2;
+  while (ncta < most && items > static_cast<int64_t>(ncta) * kMaxThreads) ncta *= 2;
+  if (ncta == 1) p.in_place = 0;  // the block's own barriers are enough
   const size_t smem = static_cast<size_t>(num_requests) * 4 * sizeof(int32_t);
-  const cudaError_t e = cudaFuncSetAttribute(paged_schedule_kernel,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kMaxRequests * 4 * static_cast<int>(sizeof(int32_t)));
-  if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  const int64_t per = ceil_div64(num_requests, threads);
+  const auto kernel = per <= 1 ? paged_schedule_kernel<1> : per <= 2 ? paged_schedule_kernel<2>
+                    : per <= 4 ? paged_schedule_kernel<4> : paged_schedule_kernel<kMaxRequests / kMaxThreads>;
+  if (smem > 48 * 1024 - 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kMaxRequests * 4 * static_cast<int>(sizeof(int32_t)));
+    if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ncta);
   cfg.blockDim = dim3(threads);
@@ -311,13 +364,13 @@ extern "C" int b200moe_paged_schedule(const int32_t* context_lens, const int32_t
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ncta;
+  attr[0].val.clusterDim.x = p.in_place ? ncta : 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, paged_schedule_kernel, p);
+  cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch(name);
 }
