@@ -45,9 +45,13 @@ struct Params {
   FastDiv by_block;
 };
 
-template <typename T> struct Row;   // how a warp holds rows of 128 elements in 16-byte pieces
+// How a thread holds a 16-byte piece of a row.  Sizes (|x|) are compared as integers, two 16-bit ones at
+// once: the order of the bits is the order of the values.
+template <typename T> struct Row;
 template <> struct Row<__nv_bfloat16> {
   static constexpr int kElems = 8;
+  static constexpr uint32_t kInfinity = 0x7f80;
+  __device__ static uint32_t size_bits(uint32_t size) { return size << 16; }  // as fp32
   __device__ static void up(uint4 v, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -59,6 +63,10 @@ template <> struct Row<__nv_bfloat16> {
 };
 template <> struct Row<__half> {
   static constexpr int kElems = 8;
+  static constexpr uint32_t kInfinity = 0x7c00;
+  __device__ static uint32_t size_bits(uint32_t size) {
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(size))));
+  }
   __device__ static void up(uint4 v, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -71,11 +79,38 @@ template <> struct Row<__half> {
 };
 template <> struct Row<float> {
   static constexpr int kElems = 4;
+  static constexpr uint32_t kInfinity = 0x7f800000;
+  __device__ static uint32_t size_bits(uint32_t size) { return size; }
   __device__ static void up(uint4 v, float (&x)[4]) {
     x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y);
     x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
   }
 };
+
+// The larger of `size` and the sizes in `v`; 16-bit sizes are kept two to a word.
+template <typename T>
+__device__ __forceinline__ uint32_t larger_size(uint32_t size, uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    size = sizeof(T) == 2 ? __vmaxu2(size, w[i] & 0x7fff7fffu) : max(size, w[i] & 0x7fffffffu);
+  return size;
+}
+// `v` with zeros in place of infinities and NaN.
+template <typename T>
+__device__ uint4 finite_only(uint4 v) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if ((w[i] & 0x7fffu) >= Row<T>::kInfinity) w[i] &= 0xffff0000u;
+      if (((w[i] >> 16) & 0x7fffu) >= Row<T>::kInfinity) w[i] &= 0xffffu;
+    } else if ((w[i] & 0x7fffffffu) >= Row<T>::kInfinity) {
+      w[i] = 0;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Slot of token `i`; -1 when it has none, or one outside the cache.
 __device__ __forceinline__ int32_t slot_of(const Params& p, int64_t i) {
@@ -107,7 +142,6 @@ __device__ void store_run(const Params& p, const Side& side, int head, int64_t f
 
   uint4 held[kU];
   int32_t slot[kU];
-  uint32_t amax = 0, begins = 0;
   auto load = [&](int64_t w) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -119,34 +153,36 @@ __device__ void store_run(const Params& p, const Side& side, int head, int64_t f
       }
     }
   };
-  for (int64_t w = 0; w < len; w += kWindow) {
-    load(w);
+  // The run's largest size over the group; infinities and NaN do not count in the second form, which is
+  // only needed when the first has met one.
+  int begins = 0;
+  auto largest = [&](bool only_finite) {
+    uint32_t size = 0;
+    for (int64_t w = 0; w < len; w += kWindow) {
+      if (!only_finite || len > kWindow) load(w);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (slot[u] < 0) continue;
-      if (slot[u] == page_slot) begins = 1;
-      float x[Row<T>::kElems];
-      Row<T>::up(held[u], x);
-#pragma unroll
-      for (int j = 0; j < Row<T>::kElems; ++j) {
-        const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-        amax = max(amax, b < 0x7f800000u ? b : 0u);  // infinities and NaN do not count
+      for (int u = 0; u < kU; ++u) {
+        if (slot[u] < 0) continue;
+        size = larger_size<T>(size, only_finite ? finite_only<T>(held[u]) : held[u]);
+        begins |= slot[u] == page_slot;
       }
     }
-  }
-  amax = __reduce_max_sync(0xffffffffu, amax);
-  begins = __reduce_max_sync(0xffffffffu, begins);
-  if (kGroupWarps > 1) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) { s_red[warp] = amax; s_red[kWarps + warp] = begins; }
-    __syncthreads();
+    if (sizeof(T) == 2) size = max(size & 0xffffu, size >> 16);
+    size = __reduce_max_sync(0xffffffffu, size);
+    if (kGroupWarps == 1) {
+      begins = __any_sync(0xffffffffu, begins);
+    } else {
+      begins = __syncthreads_or(begins);  // also: s_red has been read
+      if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = size;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kGroupWarps; ++i) {
-      amax = max(amax, s_red[i]);
-      begins = max(begins, s_red[kWarps + i]);
+      for (int i = 0; i < kGroupWarps; ++i) size = max(size, s_red[i]);
     }
-  }
-  const float needed = scale_for(amax);
+    return size;
+  };
+  uint32_t size = largest(false);
+  if (size >= Row<T>::kInfinity) size = largest(true);
+  const float needed = scale_for(Row<T>::size_bits(size));
   const float scale = begins ? needed : fmaxf(needed, old);
   if (!begins && scale > old) {
     // The page's old codes under the new scale, rows of this run included (they are overwritten below).
@@ -187,7 +223,7 @@ paged_store_fp8_kernel(const Params p) {
   __shared__ int s_begin[kMaxSegment], s_begin_page[kMaxSegment], s_page[kMaxSegment], s_long[kMaxSegment];
   __shared__ int s_num_begin, s_num_long, s_at;
   __shared__ int s_last[kWarps];
-  __shared__ uint32_t s_red[2 * kWarps];
+  __shared__ uint32_t s_red[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.x >> 1;
   const Side side = blockIdx.x & 1 ? p.value : p.key;
