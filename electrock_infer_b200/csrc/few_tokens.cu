@@ -9,18 +9,21 @@
 // The grouped GEMMs of this library pad every expert to 128 rows and go through six launches; with a few
 // tokens all that counts is to read the weights of the experts that were hit, once, at the rate of HBM:
 // 6 * H * I bytes an expert.  So the weights are the 16-row operand of m16n8k16 and the tokens its 8
-// columns; a tile is 16 weight rows with the whole contraction, split over the eight warps of a CTA.  Each
-// warp streams 16 x 128 weights per step through a ring of its own (asynchronous 16-byte copies, 20 KiB a
-// warp, 160 KiB an SM in flight), never waiting for another warp except to add up a finished tile.  Tiles
-// are dealt round-robin; that some CTAs get one more does not cost much, because an SM alone can
-// draw well over 1/148 of the HBM rate.
+// columns; a tile is 16 or 32 weight rows with the whole contraction, split over the eight warps of a CTA.
+// Each warp streams 4 KiB of weights per step, with the tokens' elements that belong to them, through a ring of
+// its own (asynchronous 16-byte copies, 192 KiB an SM), never waiting for another warp except to add up a
+// finished tile.  Tiles are dealt round-robin; that some CTAs get one more does not cost much,
+// because an SM alone can draw well over 1/148 of the HBM rate.
 //
 // * The contraction index may be permuted at will, so fragments are 16-byte reads of eight consecutive
-//   elements: of the weights from shared memory (columns swizzled by the row's parity: no bank
-//   conflicts), of the tokens straight from global memory (L1 and L2 hold them).
-// * A tile of kernel 1 is 8 gate rows over the 8 matching up rows, so that gate and up of one
+//   elements from shared memory (pieces swizzled by the row's parity: no bank conflicts).
+// * A tile of kernel 1 has 8 gate rows over the 8 matching up rows in each 16, so that gate and up of one
 //   element meet in one lane's accumulators.
-// * Tokens that are not routed to a tile's expert are zero columns: nothing is loaded for them.
+// * Only the tokens that are routed to a tile's expert are copied; the columns of the others are zeros that
+//   are not read from anywhere, and products with eight such columns are left out.  A stage has room
+//   for 16 tokens: an expert with more is gone through twice, its weights then coming from L2.
+// * Up to 8 tokens take 16-row tiles (the finest deal); more take 32-row tiles, which halve the copies of
+//   tokens per weight.
 // * act is kept as the sum of two bf16 numbers (16 bits of mantissa): kernel 2 multiplies both by
 //   the weights and adds in fp32, so that the only rounding that shows is the output's.
 // * Kernel 2 is launched with programmatic stream serialisation and fills its rings with w2 before it
@@ -36,11 +39,9 @@ constexpr int kExperts = 8;
 constexpr int kMaxTokens = 32;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;                        // weight rows of a tile
-constexpr int kStep = 128;                       // contraction elements of a ring stage
-constexpr int kStages = 5;
-constexpr int kStageBytes = kRows * kStep * 2;   // 4 KiB
-constexpr int kRingBytes = kWarps * kStages * kStageBytes;  // 160 KiB
+constexpr int kWeightBytes = 4096;     // weights of a ring stage
+constexpr int kGroup = 16;             // tokens of a ring stage
+constexpr int kRingBytes = 192 * 1024;
 
 struct Params {
   const __nv_bfloat16* x;
@@ -51,11 +52,17 @@ struct Params {
   int tokens, hidden, inter, logits_dtype, renormalize;
 };
 
+// Experts that were hit, in ascending order, and their tokens.
 struct Routing {
-  int active[kExperts];                 // the experts that were hit, ascending
   int num_active;
-  int8_t pair[kExperts][kMaxTokens];    // pair index of (expert, token), -1: not routed
+  int expert[kExperts];                 // number of the a-th active expert
+  int count[kExperts];                  // its tokens
+  int begin[kExperts + 1];              // prefix of (units * groups of tokens), see the kernel
+  int8_t token[kExperts][kMaxTokens];   // its tokens, ascending
+  int8_t rank[kExperts][kMaxTokens];    // place of a token in that list, -1: not routed to it
+  int8_t pair[kExperts][kMaxTokens];    // index of the pair, by token
   float weight[kExperts][kMaxTokens];
+  uint8_t tiles[kExperts][2];           // column tiles that hold a token of group 0, 1
 };
 
 __device__ __forceinline__ float load_logit(const void* p, int dtype, int i) {
@@ -65,7 +72,8 @@ __device__ __forceinline__ float load_logit(const void* p, int dtype, int i) {
 }
 
 // Softmax and top-2 of up to 32 tokens, one lane each (one warp).  Equal logits: the lower index wins.
-__device__ void route(const Params& p, Routing& r) {
+// `units`: tiles or steps of one expert, of which the sequence that r.begin divides is made.
+__device__ void route(const Params& p, Routing& r, int units) {
   const int t = threadIdx.x;
   int first = -1, second = -1;
   float w1 = 0.f, w2 = 0.f;
@@ -91,195 +99,330 @@ __device__ void route(const Params& p, Routing& r) {
     w1 = 1.f / sum;
     w2 = e2 / sum;
   }
-  int n = 0;
+  int n = 0, at = 0;
 #pragma unroll
   for (int e = 0; e < kExperts; ++e) {
     const int slot = first == e ? 0 : second == e ? 1 : -1;
-    r.pair[e][t] = static_cast<int8_t>(slot < 0 ? -1 : 2 * t + slot);
-    r.weight[e][t] = slot == 0 ? w1 : w2;
-    if (__any_sync(0xffffffffu, slot >= 0)) {
-      if (t == 0) r.active[n] = e;
-      ++n;
+    const uint32_t hit = __ballot_sync(0xffffffffu, slot >= 0);
+    if (hit == 0) continue;
+    const int rank = __popc(hit & ((1u << t) - 1));
+    if (slot >= 0) r.token[n][rank] = static_cast<int8_t>(t);
+    r.rank[n][t] = static_cast<int8_t>(slot < 0 ? -1 : rank);
+    r.pair[n][t] = static_cast<int8_t>(2 * t + slot);
+    r.weight[n][t] = slot == 0 ? w1 : w2;
+    const int count = __popc(hit);
+    uint32_t tiles[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kMaxTokens / 8; ++i)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (__any_sync(0xffffffffu, slot >= 0 && t / 8 == i && rank / kGroup == q)) tiles[q] |= 1u << i;
+    if (t == 0) {
+      r.expert[n] = e;
+      r.count[n] = count;
+      r.begin[n] = at;
+      r.tiles[n][0] = static_cast<uint8_t>(tiles[0]);
+      r.tiles[n][1] = static_cast<uint8_t>(tiles[1]);
     }
+    at += units * ((count + kGroup - 1) / kGroup);
+    ++n;
   }
-  if (t == 0) r.num_active = n;
+  if (t == 0) {
+    r.num_active = n;
+    r.begin[n] = at;
+  }
 }
 
-// Byte offset of 16-byte column `col` of row `row` in a stage of 256-byte rows.
-__device__ __forceinline__ uint32_t stage_offset(int row, int col) {
-  return static_cast<uint32_t>(row * kStep * 2 + ((col ^ ((row & 1) << 2)) << 4));
+// A place in the sequence of (active expert, unit, group of tokens): units are tiles of kernel 1 and
+// contraction steps of kernel 2, the groups of one unit follow one another.
+struct Place {
+  int a, unit, group;
+  // Moves forward to position `at` of the sequence.
+  __device__ __forceinline__ void seek(const Routing& r, int at) {
+    while (at >= r.begin[a + 1]) ++a;
+    const int rest = at - r.begin[a];
+    const bool two = r.count[a] > kGroup;
+    unit = two ? rest >> 1 : rest;
+    group = two ? rest & 1 : 0;
+  }
+};
+
+// kNT = tiles of 8 tokens, kRT = tiles of 16 weight rows.
+template <int kNT, int kRT, bool kDown>
+struct Shape {
+  static constexpr int kStep = 128 / kRT;                      // contraction elements of a stage
+  static constexpr int kPieces = kStep / 8;                    // 16-byte pieces of a weight row
+  static constexpr int kParts = kDown ? 2 : 1;                 // numbers that an element is the sum of
+  static constexpr int kSlots = kNT == 1 ? 8 : kGroup;         // tokens that a stage has room for
+  static constexpr int kTokenPieces = kPieces * kParts;
+  static constexpr int kStageBytes = kWeightBytes + kSlots * kTokenPieces * 16;
+  static constexpr int kStages = kRingBytes / kWarps / kStageBytes;
+  static constexpr int kRows = 16 * kRT;
+  static constexpr int kSets = kNT * kRT == 1 ? 2 : 1;         // accumulator sets, against dependent products
+  static_assert(kStages >= 2, "the ring is too small");
+};
+
+// Byte offsets in a stage: piece `col` of weight row `row`; piece `col`, part `part` of token slot `slot`.
+// Two rows or slots of different parity never meet in a bank where a quarter of a warp reads them.
+template <typename S> __device__ __forceinline__ uint32_t weight_offset(int row, int col) {
+  return static_cast<uint32_t>((row * S::kPieces + (col ^ ((row & 1) << 2))) * 16);
+}
+template <typename S> __device__ __forceinline__ uint32_t token_offset(int slot, int piece) {
+  const int mixed = S::kParts == 2 ? piece ^ (slot & 1) : piece ^ ((slot & 1) << 2);
+  return static_cast<uint32_t>(kWeightBytes + (slot * S::kTokenPieces + mixed) * 16);
 }
 
-template <int kNT, bool kDown>  // kNT = tiles of 8 tokens
+template <int kNT, int kRT, bool kDown>
 __global__ void __launch_bounds__(kThreads, 1)
 few_tokens_kernel(const Params p) {
+  using S = Shape<kNT, kRT, kDown>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Routing r;
-  __shared__ float4 s_sum[2][kWarps][kNT][32];
+  __shared__ float4 s_sum[kNT * kRT <= 2 ? 2 : 1][kWarps][kNT * kRT][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int K = kDown ? p.inter : p.hidden;
+  const int steps = (K + S::kStep - 1) / S::kStep;                             // of one expert
+  const int expert_tiles = kDown ? p.hidden / S::kRows : p.inter / (S::kRows / 2);
   // Kernel 2 may look at the logits before kernel 1 is through: kernel 1 lets it start only after its own
   // wait, that is after everything before it in the stream has finished.
   if (!kDown) pdl_wait();
-  if (warp == 0) route(p, r);
+  if (warp == 0) route(p, r, kDown ? steps : expert_tiles);
   __syncthreads();
   pdl_launch_dependents();
 
-  const int K = kDown ? p.inter : p.hidden;
-  const int steps = (K + kStep - 1) / kStep;                              // of one expert
-  const int chunks = kDown ? r.num_active * steps : steps;                // of one tile
-  const int expert_tiles = kDown ? p.hidden / kRows : p.inter / (kRows / 2);
-  const int tiles = kDown ? expert_tiles : r.num_active * expert_tiles;
+  const int chunks = kDown ? r.begin[r.num_active] : steps;                    // of one tile
+  const int tiles = kDown ? expert_tiles : r.begin[r.num_active];
   const int my_chunks = chunks > warp ? (chunks - warp + kWarps - 1) / kWarps : 0;  // of one tile
-  const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
+  const uint32_t ring = smem_addr(smem) + warp * S::kStages * S::kStageBytes;
   const int64_t row_bytes = static_cast<int64_t>(K) * 2;
-  const int64_t up_gap = kDown ? 0 : static_cast<int64_t>(p.inter - kRows / 2) * row_bytes;
+  const int64_t up_gap = kDown ? 0 : static_cast<int64_t>(p.inter - 8) * row_bytes;  // from gate rows to up rows
 
-  // Issues the copies of chunk `c` of tile `tile`: 16 weight rows x 128 elements, zeros past K.
-  auto issue = [&](int tile, int c, int stage) {
-    if (tile < tiles) {
-      const int a = kDown ? c / steps : tile / expert_tiles;
-      const int k0 = (kDown ? c - a * steps : c) * kStep;
-      const int row0 = kDown ? tile * kRows : (tile - a * expert_tiles) * (kRows / 2);
-      const int64_t expert_rows = kDown ? p.hidden : 2 * static_cast<int64_t>(p.inter);
-      const int row = lane >> 4, col = lane & 15;
-      const int bytes = k0 + col * 8 < K ? 16 : 0;
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.w) +
-                           (r.active[a] * expert_rows + row0 + row) * row_bytes + (bytes ? (k0 + col * 8) * 2 : 0);
+  // Copies of the weights of chunk `c` of a tile: kRows rows x kStep elements, zeros past K.
+  auto issue_weights = [&](int tile, const Place& at, int step, uint32_t to) {
+    const int k0 = step * S::kStep;
+    const int row0 = kDown ? tile * S::kRows : at.unit * (S::kRows / 2);
+    const int64_t expert_rows = kDown ? p.hidden : 2 * static_cast<int64_t>(p.inter);
+    constexpr int kRowsAtOnce = 32 / S::kPieces;   // 2 or 4, of one row tile's eight upper or lower rows
+    const int row = lane / S::kPieces, col = lane % S::kPieces;
+    const int bytes = k0 + col * 8 < K ? 16 : 0;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(p.w) +
+                         (r.expert[at.a] * expert_rows + row0 + row) * row_bytes + (bytes ? (k0 + col * 8) * 2 : 0);
 #pragma unroll
-      for (int j = 0; j < kRows / 2; ++j)
-        cp_async_16(ring + stage * kStageBytes + stage_offset(row + 2 * j, col),
-                    src + 2 * j * row_bytes + (j >= kRows / 4 ? up_gap : 0), bytes);
+    for (int j = 0; j < S::kRows / kRowsAtOnce; ++j) {
+      const int base = j * kRowsAtOnce;            // rows base + row of the tile
+      // Kernel 1: rows 16 m + 0..7 are gate rows 8 m + 0..7, rows 16 m + 8..15 the same up rows.
+      const int from = kDown ? base : base / 16 * 8 + base % 8;
+      cp_async_16(to + weight_offset<S>(base + row, col),
+                  src + from * row_bytes + (!kDown && base % 16 >= 8 ? up_gap + 8 * row_bytes : 0), bytes);
+    }
+  };
+  // Copies of the group's tokens that belong to them.
+  auto issue_tokens = [&](const Place& at, int step, uint32_t to) {
+    const int live = min(r.count[at.a] - at.group * kGroup, kGroup);
+    const int k0 = step * S::kStep;
+#pragma unroll
+    for (int i = 0; i < S::kSlots * S::kTokenPieces / 32; ++i) {
+      const int index = i * 32 + lane;
+      const int slot = index / S::kTokenPieces, piece = index % S::kTokenPieces;
+      if (slot < live) {
+        const int token = r.token[at.a][at.group * kGroup + slot];
+        const int k = k0 + piece / S::kParts * 8;
+        const int bytes = k < K ? 16 : 0;
+        const void* src;
+        if constexpr (kDown) {
+          src = p.act + (static_cast<int64_t>(r.pair[at.a][token]) * (p.inter / 8) + (bytes ? k / 8 : 0)) * 2 +
+                piece % S::kParts;
+        } else {
+          src = p.x + static_cast<int64_t>(token) * p.hidden + (bytes ? k : 0);
+        }
+        cp_async_16(to + token_offset<S>(slot, piece), src, bytes);
+      }
+    }
+  };
+
+  // The warp's chunks of all its tiles as one sequence, of which `ahead` is the next to be issued.
+  Place ahead = {0, 0, 0};
+  int ahead_tile = my_chunks ? blockIdx.x : tiles, ahead_chunk = 0, filled = 0;
+  auto ahead_step = [&]() {  // seeks the place, returns the contraction step
+    const int c = warp + ahead_chunk * kWarps;
+    if (kDown) {
+      if (ahead_chunk == 0) ahead.a = 0;
+      ahead.seek(r, c);
+      return ahead.unit;
+    }
+    if (ahead_chunk == 0) ahead.seek(r, ahead_tile);
+    return c;
+  };
+  auto advance = [&]() {
+    filled = filled + 1 == S::kStages ? 0 : filled + 1;
+    if (++ahead_chunk >= my_chunks) { ahead_chunk = 0; if (ahead_tile < tiles) ahead_tile += gridDim.x; }
+  };
+  auto issue_next = [&]() {
+    if (ahead_tile < tiles) {
+      const int step = ahead_step();
+      const uint32_t to = ring + filled * S::kStageBytes;
+      issue_weights(ahead_tile, ahead, step, to);
+      issue_tokens(ahead, step, to);
     }
     cp_async_commit();
+    advance();
   };
-
-  // The warp's chunks of all its tiles, as one sequence.
-  int ahead_tile = my_chunks ? blockIdx.x : tiles, ahead = 0, filled = 0;
-  auto issue_next = [&]() {
-    issue(ahead_tile, warp + ahead * kWarps, filled);
-    filled = filled + 1 == kStages ? 0 : filled + 1;
-    if (++ahead >= my_chunks) { ahead = 0; if (ahead_tile < tiles) ahead_tile += gridDim.x; }
-  };
+  if constexpr (kDown) {
+    // Weights first, then, once kernel 1 is through, the activations that go with them.
+    const int tile0 = ahead_tile;
+    for (int s = 0; s < S::kStages - 1; ++s) {
+      if (ahead_tile < tiles) {
+        const int step = ahead_step();
+        issue_weights(ahead_tile, ahead, step, ring + filled * S::kStageBytes);
+      }
+      advance();
+    }
+    ahead_tile = tile0; ahead_chunk = 0; filled = 0; ahead = {0, 0, 0};
+    pdl_wait();
+    for (int s = 0; s < S::kStages - 1; ++s) {
+      if (ahead_tile < tiles) {
+        const int step = ahead_step();
+        issue_tokens(ahead, step, ring + filled * S::kStageBytes);
+      }
+      cp_async_commit();
+      advance();
+    }
+  } else {
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue_next();
-  if (kDown) pdl_wait();
+    for (int s = 0; s < S::kStages - 1; ++s) issue_next();
+  }
 
   int stage = 0, parity = 0;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, parity ^= 1) {
-    float acc[kNT][4];
+  Place here = {0, 0, 0};
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    float acc[S::kSets][kRT][kNT][4];
 #pragma unroll
-    for (int n = 0; n < kNT; ++n)
+    for (int s = 0; s < S::kSets; ++s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
-    const int tile_expert = kDown ? 0 : r.active[tile / expert_tiles];
-
-    for (int i = 0; i < my_chunks; ++i) {
-      const int c = warp + i * kWarps;
-      const int a = kDown ? c / steps : 0;
-      const int k0 = (kDown ? c - a * steps : c) * kStep;
-      const int e = kDown ? r.active[a] : tile_expert;
-      // The tokens' side of the products: eight elements from k0 + kk * 32 + t * 8.
-      uint4 b[kStep / 32][kNT][kDown ? 2 : 1];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        const int pair = r.pair[e][n * 8 + g];
-#pragma unroll
-        for (int kk = 0; kk < kStep / 32; ++kk) {
-          const int k = k0 + kk * 32 + t * 8;
-          const bool live = pair >= 0 && k < K;
-          if constexpr (kDown) {
-            const uint4* at = p.act + (static_cast<int64_t>(pair) * (p.inter / 8) + k / 8) * 2;
-            b[kk][n][0] = live ? at[0] : make_uint4(0, 0, 0, 0);
-            b[kk][n][1] = live ? at[1] : make_uint4(0, 0, 0, 0);
-          } else {
-            b[kk][n][0] = live ? __ldg(reinterpret_cast<const uint4*>(
-                                     p.x + static_cast<int64_t>(n * 8 + g) * p.hidden + k))
-                               : make_uint4(0, 0, 0, 0);
-          }
-        }
-      }
-      issue_next();
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
-      const uint32_t at = ring + stage * kStageBytes;
-#pragma unroll
-      for (int kk = 0; kk < kStep / 32; ++kk) {
-        const uint4 lo = lds_16(at + stage_offset(g, kk * 4 + t)), hi = lds_16(at + stage_offset(g + 8, kk * 4 + t));
-        const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+      for (int m = 0; m < kRT; ++m)
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
-          for (int h = 0; h < (kDown ? 2 : 1); ++h) {
-            Mma<__nv_bfloat16>::run(acc[n], a0, b[kk][n][h].x, b[kk][n][h].y);
-            Mma<__nv_bfloat16>::run(acc[n], a1, b[kk][n][h].z, b[kk][n][h].w);
+          for (int j = 0; j < 4; ++j) acc[s][m][n][j] = 0.f;
+    if (kDown) here = {0, 0, 0}; else here.seek(r, tile);
+
+    for (int i = 0; i < my_chunks; ++i) {
+      if (kDown) here.seek(r, warp + i * kWarps);
+      issue_next();
+      cp_async_wait<S::kStages - 1>();
+      __syncwarp();
+      const uint32_t at = ring + stage * S::kStageBytes;
+      int slot[kNT];  // where the lane's token of each column tile stands in the stage; -1: a zero column
+      const uint32_t used = r.tiles[here.a][here.group];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        const int rank = r.rank[here.a][n * 8 + g] - here.group * kGroup;
+        slot[n] = rank < kGroup ? rank : -1;
+      }
+#pragma unroll
+      for (int kk = 0; kk < S::kStep / 32; ++kk) {
+        uint32_t a0[kRT][4], a1[kRT][4];
+#pragma unroll
+        for (int m = 0; m < kRT; ++m) {
+          const uint4 lo = lds_16(at + weight_offset<S>(m * 16 + g, kk * 4 + t));
+          const uint4 hi = lds_16(at + weight_offset<S>(m * 16 + g + 8, kk * 4 + t));
+          a0[m][0] = lo.x; a0[m][1] = hi.x; a0[m][2] = lo.y; a0[m][3] = hi.y;
+          a1[m][0] = lo.z; a1[m][1] = hi.z; a1[m][2] = lo.w; a1[m][3] = hi.w;
+        }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          if (kNT > 1 && !(used >> n & 1)) continue;
+#pragma unroll
+          for (int h = 0; h < S::kParts; ++h) {
+            uint4 b = make_uint4(0, 0, 0, 0);
+            if (slot[n] >= 0) b = lds_16(at + token_offset<S>(slot[n], (kk * 4 + t) * S::kParts + h));
+#pragma unroll
+            for (int m = 0; m < kRT; ++m) {
+              Mma<__nv_bfloat16>::run(acc[0][m][n], a0[m], b.x, b.y);
+              Mma<__nv_bfloat16>::run(acc[S::kSets - 1][m][n], a1[m], b.z, b.w);
+            }
           }
+        }
       }
       __syncwarp();  // the stage is refilled by a later iteration's copies
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
     }
 
-    // Add the warps up, in their order; the two buffers make one barrier per tile enough.
+    // Add the warps up, in their order.
+    if (sizeof(s_sum) / sizeof(s_sum[0]) == 1) __syncthreads();  // with two buffers, one barrier per tile is enough
 #pragma unroll
-    for (int n = 0; n < kNT; ++n) s_sum[parity][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+    for (int m = 0; m < kRT; ++m)
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        float4 v = make_float4(acc[0][m][n][0], acc[0][m][n][1], acc[0][m][n][2], acc[0][m][n][3]);
+        if (S::kSets == 2) {
+          v.x += acc[S::kSets - 1][m][n][0]; v.y += acc[S::kSets - 1][m][n][1];
+          v.z += acc[S::kSets - 1][m][n][2]; v.w += acc[S::kSets - 1][m][n][3];
+        }
+        s_sum[parity][warp][m * kNT + n][lane] = v;
+      }
     __syncthreads();
-    if (warp < kNT) {
+    if (warp < kNT * kRT) {
       float4 v = s_sum[parity][0][warp][lane];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) {
         const float4 o = s_sum[parity][w][warp][lane];
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
-      // Elements (row g, tokens 2 t, 2 t + 1) and (row g + 8, the same tokens).
+      const int m = warp / kNT, n = warp % kNT;
+      // Elements (row g, tokens 2 t, 2 t + 1) and (row g + 8, the same tokens) of row tile m.
       const float top[2] = {v.x, v.y}, bottom[2] = {v.z, v.w};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int token = warp * 8 + 2 * t + c;
+        const int token = n * 8 + 2 * t + c;
         if constexpr (kDown) {
           if (token < p.tokens) {
-            __nv_bfloat16* o = p.out + static_cast<int64_t>(token) * p.hidden + tile * kRows + g;
+            __nv_bfloat16* o = p.out + static_cast<int64_t>(token) * p.hidden + tile * S::kRows + m * 16 + g;
             o[0] = __float2bfloat16_rn(top[c]);
             o[8] = __float2bfloat16_rn(bottom[c]);
           }
         } else {
-          const int pair = r.pair[tile_expert][token];
-          if (pair >= 0) {
-            const int group = tile % expert_tiles;  // eight elements of the expert's width
-            const float value = r.weight[tile_expert][token] * (top[c] / (1.f + expf(-top[c])) * bottom[c]);
+          const int rank = r.rank[here.a][token];
+          if (rank >= 0 && rank / kGroup == here.group) {
+            const float value = r.weight[here.a][token] * (top[c] / (1.f + expf(-top[c])) * bottom[c]);
             const __nv_bfloat16 high = __float2bfloat16_rn(value);
             const float rest = value - __bfloat162float(high);
             __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(
-                p.act + (static_cast<int64_t>(pair) * expert_tiles + group) * 2);
+                p.act + (static_cast<int64_t>(r.pair[here.a][token]) * (p.inter / 8) + here.unit * kRT + m) * 2);
             o[g] = high;
             o[8 + g] = __float2bfloat16_rn(rest);
           }
         }
       }
     }
+    if (sizeof(s_sum) / sizeof(s_sum[0]) == 2) parity ^= 1;
   }
   cp_async_wait<0>();
 }
 
+template <int kNT, int kRT, bool kDown>
+int launch(const Params& p, int64_t tiles, cudaStream_t st) {
+  const char* name = "moe_few_tokens";
+  const auto kernel = few_tokens_kernel<kNT, kRT, kDown>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  const int64_t sms = sm_count();
+  launch_pdl(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), dim3(kThreads), kRingBytes, st, p);
+  return check_launch(name);
+}
+
+// 32-row tiles where there are more than 8 tokens and the sizes allow it.
 template <int kNT>
 int launch(Params p, const void* w13, const void* w2, cudaStream_t st) {
-  const char* name = "moe_few_tokens";
-  for (int down = 0; down < 2; ++down) {
-    const cudaError_t e =
-        down ? cudaFuncSetAttribute(few_tokens_kernel<kNT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes)
-             : cudaFuncSetAttribute(few_tokens_kernel<kNT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-    if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
-  }
   const int experts_hit = 2 * p.tokens < kExperts ? 2 * p.tokens : kExperts;
-  const int64_t up_tiles = static_cast<int64_t>(experts_hit) * p.inter / (kRows / 2), down_tiles = p.hidden / kRows;
-  const int64_t sms = sm_count();
+  constexpr int kRT = kNT == 1 ? 1 : 2;
+  const bool wide_up = p.inter % (8 * kRT) == 0, wide_down = p.hidden % (16 * kRT) == 0;
   p.w = static_cast<const __nv_bfloat16*>(w13);
-  launch_pdl(few_tokens_kernel<kNT, false>, dim3(static_cast<unsigned>(up_tiles < sms ? up_tiles : sms)), dim3(kThreads),
-             kRingBytes, st, p);
-  if (int rc = check_launch(name)) return rc;
+  const int64_t up_tiles = static_cast<int64_t>(experts_hit) * p.inter / 8;
+  if (int rc = wide_up ? launch<kNT, kRT, false>(p, up_tiles / kRT, st) : launch<kNT, 1, false>(p, up_tiles, st)) return rc;
   p.w = static_cast<const __nv_bfloat16*>(w2);
-  launch_pdl(few_tokens_kernel<kNT, true>, dim3(static_cast<unsigned>(down_tiles < sms ? down_tiles : sms)), dim3(kThreads),
-             kRingBytes, st, p);
-  return check_launch(name);
+  return wide_down ? launch<kNT, kRT, true>(p, p.hidden / (16 * kRT), st) : launch<kNT, 1, true>(p, p.hidden / 16, st);
 }
 
 }  // namespace
@@ -329,10 +472,7 @@ extern "C" int b200moe_few_tokens(const void* hidden_states, const void* gating_
   p.logits_dtype = logits_dtype;
   p.renormalize = renormalize;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch ((num_tokens + 7) / 8) {
-    case 1: return launch<1>(p, w13, w2, st);
-    case 2: return launch<2>(p, w13, w2, st);
-    case 3: return launch<3>(p, w13, w2, st);
-    default: return launch<4>(p, w13, w2, st);
-  }
+  if (num_tokens <= 8) return launch<1>(p, w13, w2, st);
+  if (num_tokens <= 16) return launch<2>(p, w13, w2, st);
+  return launch<4>(p, w13, w2, st);
 }
