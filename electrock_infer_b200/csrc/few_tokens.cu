@@ -15,13 +15,13 @@
 // finished tile.  Tiles are dealt round-robin; that some CTAs get one more does not cost much,
 // because an SM alone can draw well over 1/148 of the HBM rate.
 //
-// * The contraction index may be permuted at will, so fragments are 16-byte reads of eight consecutive
-//   elements from shared memory (pieces swizzled by the row's parity: no bank conflicts).
+// * Fragments come from matrix loads, whose registers are the products' operands as they are (16-byte
+//   reads of a row and a permuted contraction index need as many reads, and four moves for each product).
 // * A tile of kernel 1 has 8 gate rows over the 8 matching up rows in each 16, so that gate and up of one
 //   element meet in one lane's accumulators.
-// * Only the tokens that are routed to a tile's expert are copied; the columns of the others are zeros that
-//   are not read from anywhere, and products with eight such columns are left out.  A stage has room
-//   for 16 tokens: an expert with more is gone through twice, its weights then coming from L2.
+// * Only the tokens that are routed to a tile's expert are copied and multiplied: columns are their places
+//   in the expert's list.  A stage has room for 16; an expert with more is gone through twice, its weights
+//   then coming from L2.  Kernel 2 adds its columns to the tokens' sums whenever the expert changes.
 // * Up to 8 tokens take 16-row tiles (the finest deal); more take 32-row tiles, which halve the copies of
 //   tokens per weight.
 // * act is kept as the sum of two bf16 numbers (16 bits of mantissa): kernel 2 multiplies both by
@@ -30,6 +30,8 @@
 //   waits for kernel 1.
 //
 // The reference runs the same batch through its general path (layers/moe/fused_moe.py:170-293).
+#include <type_traits>
+
 #include "warp_mma.cuh"
 
 namespace b200moe {
@@ -59,10 +61,8 @@ struct Routing {
   int count[kExperts];                  // its tokens
   int begin[kExperts + 1];              // prefix of (units * groups of tokens), see the kernel
   int8_t token[kExperts][kMaxTokens];   // its tokens, ascending
-  int8_t rank[kExperts][kMaxTokens];    // place of a token in that list, -1: not routed to it
-  int8_t pair[kExperts][kMaxTokens];    // index of the pair, by token
-  float weight[kExperts][kMaxTokens];
-  uint8_t tiles[kExperts][2];           // column tiles that hold a token of group 0, 1
+  int8_t pair[kExperts][kMaxTokens];    // the pairs' indices, in the same order
+  float weight[kExperts][kMaxTokens];   // and their routing weights
 };
 
 __device__ __forceinline__ float load_logit(const void* p, int dtype, int i) {
@@ -106,23 +106,16 @@ __device__ void route(const Params& p, Routing& r, int units) {
     const uint32_t hit = __ballot_sync(0xffffffffu, slot >= 0);
     if (hit == 0) continue;
     const int rank = __popc(hit & ((1u << t) - 1));
-    if (slot >= 0) r.token[n][rank] = static_cast<int8_t>(t);
-    r.rank[n][t] = static_cast<int8_t>(slot < 0 ? -1 : rank);
-    r.pair[n][t] = static_cast<int8_t>(2 * t + slot);
-    r.weight[n][t] = slot == 0 ? w1 : w2;
+    if (slot >= 0) {
+      r.token[n][rank] = static_cast<int8_t>(t);
+      r.pair[n][rank] = static_cast<int8_t>(2 * t + slot);
+      r.weight[n][rank] = slot == 0 ? w1 : w2;
+    }
     const int count = __popc(hit);
-    uint32_t tiles[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < kMaxTokens / 8; ++i)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (__any_sync(0xffffffffu, slot >= 0 && t / 8 == i && rank / kGroup == q)) tiles[q] |= 1u << i;
     if (t == 0) {
       r.expert[n] = e;
       r.count[n] = count;
       r.begin[n] = at;
-      r.tiles[n][0] = static_cast<uint8_t>(tiles[0]);
-      r.tiles[n][1] = static_cast<uint8_t>(tiles[1]);
     }
     at += units * ((count + kGroup - 1) / kGroup);
     ++n;
@@ -133,52 +126,55 @@ __device__ void route(const Params& p, Routing& r, int units) {
   }
 }
 
-// A place in the sequence of (active expert, unit, group of tokens): units are tiles of kernel 1 and
-// contraction steps of kernel 2, the groups of one unit follow one another.
+// A warp's way through the sequence of (active expert, unit, group of tokens): units are tiles of kernel 1
+// and contraction steps of kernel 2, the groups of one unit follow one another.
 struct Place {
-  int a, unit, group;
+  int a, until, unit, group, groups;
   // Moves forward to position `at` of the sequence.
   __device__ __forceinline__ void seek(const Routing& r, int at) {
     while (at >= r.begin[a + 1]) ++a;
+    until = r.begin[a + 1];
+    groups = r.count[a] > kGroup ? 2 : 1;
     const int rest = at - r.begin[a];
-    const bool two = r.count[a] > kGroup;
-    unit = two ? rest >> 1 : rest;
-    group = two ? rest & 1 : 0;
+    unit = groups == 2 ? rest >> 1 : rest;
+    group = groups == 2 ? rest & 1 : 0;
   }
 };
 
-// kNT = tiles of 8 tokens, kRT = tiles of 16 weight rows.
-template <int kNT, int kRT, bool kDown>
+// kCT = tiles of 8 tokens that a stage has room for, kRT = tiles of 16 weight rows.
+template <int kCT, int kRT, bool kDown>
 struct Shape {
   static constexpr int kStep = 128 / kRT;                      // contraction elements of a stage
   static constexpr int kPieces = kStep / 8;                    // 16-byte pieces of a weight row
   static constexpr int kParts = kDown ? 2 : 1;                 // numbers that an element is the sum of
-  static constexpr int kSlots = kNT == 1 ? 8 : kGroup;         // tokens that a stage has room for
+  static constexpr int kSlots = 8 * kCT;                       // tokens that a stage has room for
   static constexpr int kTokenPieces = kPieces * kParts;
   static constexpr int kStageBytes = kWeightBytes + kSlots * kTokenPieces * 16;
   static constexpr int kStages = kRingBytes / kWarps / kStageBytes;
   static constexpr int kRows = 16 * kRT;
-  static constexpr int kSets = kNT * kRT == 1 ? 2 : 1;         // accumulator sets, against dependent products
+  static constexpr int kSets = kCT * kRT == 1 ? 2 : 1;         // accumulator sets, against dependent products
+  static constexpr int kMaxT = kCT == 1 ? 8 : kMaxTokens;      // tokens of the batch
+  // What the warps add up through: kernel 1 two buffers of accumulators, kernel 2 a tile per warp.
+  static constexpr int kSumFloats = kDown ? kRows * kMaxT : 2 * kRT * kCT * 32 * 4;
   static_assert(kStages >= 2, "the ring is too small");
 };
 
-// Byte offsets in a stage: piece `col` of weight row `row`; piece `col`, part `part` of token slot `slot`.
-// Two rows or slots of different parity never meet in a bank where a quarter of a warp reads them.
+// Byte offsets in a stage: piece `col` of weight row `row`; piece `piece` of token slot `slot`.  Eight rows or
+// slots in a row never meet in a bank.
 template <typename S> __device__ __forceinline__ uint32_t weight_offset(int row, int col) {
-  return static_cast<uint32_t>((row * S::kPieces + (col ^ ((row & 1) << 2))) * 16);
+  return static_cast<uint32_t>((row * S::kPieces + (col ^ (row & 7))) * 16);
 }
 template <typename S> __device__ __forceinline__ uint32_t token_offset(int slot, int piece) {
-  const int mixed = S::kParts == 2 ? piece ^ (slot & 1) : piece ^ ((slot & 1) << 2);
-  return static_cast<uint32_t>(kWeightBytes + (slot * S::kTokenPieces + mixed) * 16);
+  return static_cast<uint32_t>(kWeightBytes + (slot * S::kTokenPieces + (piece ^ (slot & 7))) * 16);
 }
 
-template <int kNT, int kRT, bool kDown>
+template <int kCT, int kRT, bool kDown>
 __global__ void __launch_bounds__(kThreads, 1)
 few_tokens_kernel(const Params p) {
-  using S = Shape<kNT, kRT, kDown>;
+  using S = Shape<kCT, kRT, kDown>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Routing r;
-  __shared__ float4 s_sum[kNT * kRT <= 2 ? 2 : 1][kWarps][kNT * kRT][32];
+  __shared__ __align__(16) float s_sum[kWarps * S::kSumFloats];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int K = kDown ? p.inter : p.hidden;
@@ -188,6 +184,8 @@ few_tokens_kernel(const Params p) {
   // wait, that is after everything before it in the stream has finished.
   if (!kDown) pdl_wait();
   if (warp == 0) route(p, r, kDown ? steps : expert_tiles);
+  if (kDown)
+    for (int i = threadIdx.x; i < kWarps * S::kSumFloats; i += kThreads) s_sum[i] = 0.f;
   __syncthreads();
   pdl_launch_dependents();
 
@@ -196,215 +194,281 @@ few_tokens_kernel(const Params p) {
   const int my_chunks = chunks > warp ? (chunks - warp + kWarps - 1) / kWarps : 0;  // of one tile
   const uint32_t ring = smem_addr(smem) + warp * S::kStages * S::kStageBytes;
   const int64_t row_bytes = static_cast<int64_t>(K) * 2;
-  const int64_t up_gap = kDown ? 0 : static_cast<int64_t>(p.inter - 8) * row_bytes;  // from gate rows to up rows
+  const int64_t expert_rows = kDown ? p.hidden : 2 * static_cast<int64_t>(p.inter);
 
-  // Copies of the weights of chunk `c` of a tile: kRows rows x kStep elements, zeros past K.
-  auto issue_weights = [&](int tile, const Place& at, int step, uint32_t to) {
-    const int k0 = step * S::kStep;
-    const int row0 = kDown ? tile * S::kRows : at.unit * (S::kRows / 2);
-    const int64_t expert_rows = kDown ? p.hidden : 2 * static_cast<int64_t>(p.inter);
-    constexpr int kRowsAtOnce = 32 / S::kPieces;   // 2 or 4, of one row tile's eight upper or lower rows
-    const int row = lane / S::kPieces, col = lane % S::kPieces;
-    const int bytes = k0 + col * 8 < K ? 16 : 0;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(p.w) +
-                         (r.expert[at.a] * expert_rows + row0 + row) * row_bytes + (bytes ? (k0 + col * 8) * 2 : 0);
+  // ---- The copying side.  The warp's chunks of all its tiles are one sequence; what a lane copies of a
+  // chunk is at fixed distances from what it copied of the last one, until the expert or the tile changes.
+  constexpr int kRowsAtOnce = 32 / S::kPieces;                     // weight rows of one copy instruction
+  constexpr int kTokenCopies = S::kSlots * S::kTokenPieces / 32;   // copy instructions of the tokens
+  const int w_row = lane / S::kPieces, w_col = lane % S::kPieces;
+  Place ahead = {0, 0, 0, 0, 1};
+  int ahead_tile = my_chunks ? blockIdx.x : tiles, ahead_chunk = 0, filled = 0;
+  int step = 0, step_by = 0;           // contraction step of the next chunk, and its increment
+  const uint8_t* w_src = nullptr;      // of the next chunk
+  const uint8_t* t_src[kTokenCopies];
+  int live = 0;                        // tokens of the group
+
+  auto locate = [&]() {  // the next chunk has another expert, group or tile than the last one
+    ahead.seek(r, kDown ? warp + ahead_chunk * kWarps : ahead_tile);
+    step = kDown ? ahead.unit : warp;
+    step_by = kDown ? kWarps / ahead.groups : kWarps;
+    const int row0 = kDown ? ahead_tile * S::kRows : ahead.unit * (S::kRows / 2);
+    w_src = reinterpret_cast<const uint8_t*>(p.w) + (r.expert[ahead.a] * expert_rows + row0 + w_row) * row_bytes +
+            (static_cast<int64_t>(step) * S::kStep + w_col * 8) * 2;
+    live = min(r.count[ahead.a] - ahead.group * kGroup, kGroup);
 #pragma unroll
-    for (int j = 0; j < S::kRows / kRowsAtOnce; ++j) {
-      const int base = j * kRowsAtOnce;            // rows base + row of the tile
-      // Kernel 1: rows 16 m + 0..7 are gate rows 8 m + 0..7, rows 16 m + 8..15 the same up rows.
-      const int from = kDown ? base : base / 16 * 8 + base % 8;
-      cp_async_16(to + weight_offset<S>(base + row, col),
-                  src + from * row_bytes + (!kDown && base % 16 >= 8 ? up_gap + 8 * row_bytes : 0), bytes);
+    for (int i = 0; i < kTokenCopies; ++i) {
+      const int slot = (i * 32 + lane) / S::kTokenPieces, piece = (i * 32 + lane) % S::kTokenPieces;
+      const int at = ahead.group * kGroup + slot;
+      const int token = slot < live ? r.token[ahead.a][at] : 0;
+      const int64_t k = static_cast<int64_t>(step) * S::kStep + piece / S::kParts * 8;
+      t_src[i] = kDown ? reinterpret_cast<const uint8_t*>(p.act) +
+                             (static_cast<int64_t>(slot < live ? r.pair[ahead.a][at] : 0) * p.inter + k) * 4 +
+                             piece % S::kParts * 16
+                       : reinterpret_cast<const uint8_t*>(p.x) + (static_cast<int64_t>(token) * p.hidden + k) * 2;
     }
   };
-  // Copies of the group's tokens that belong to them.
-  auto issue_tokens = [&](const Place& at, int step, uint32_t to) {
-    const int live = min(r.count[at.a] - at.group * kGroup, kGroup);
-    const int k0 = step * S::kStep;
+  const int64_t rows_down = kRowsAtOnce * row_bytes;
+  // Kernel 1: rows 16 m + 0..7 of a tile are gate rows 8 m + 0..7, rows 16 m + 8..15 the same up rows.
+  const int64_t gate_to_up = (p.inter - 8 + kRowsAtOnce) * row_bytes;
+  const int64_t up_to_gate = (kRowsAtOnce - p.inter) * row_bytes;
+  // kRows rows x kStep elements of weights; zeros past K.
+  auto issue_weights = [&](uint32_t to) {
+    const uint8_t* src = w_src;
+    const uint32_t dst = to + weight_offset<S>(w_row, w_col), dst_odd = to + weight_offset<S>(w_row + 4, w_col);
+    const int bytes = (step + 1) * S::kStep <= K || step * S::kStep + w_col * 8 < K ? 16 : 0;
+    if (bytes == 0) src = reinterpret_cast<const uint8_t*>(p.w);
 #pragma unroll
-    for (int i = 0; i < S::kSlots * S::kTokenPieces / 32; ++i) {
-      const int index = i * 32 + lane;
-      const int slot = index / S::kTokenPieces, piece = index % S::kTokenPieces;
+    for (int j = 0; j < S::kRows / kRowsAtOnce; ++j) {
+      const int base = j * kRowsAtOnce;  // rows base + w_row of the tile
+      if (kRowsAtOnce == 4) {
+        // Rows 4 apart differ in the swizzle, rows 8 apart do not.
+        cp_async_16((base & 4 ? dst_odd : dst) + (base & ~7) * S::kPieces * 16, src, bytes);
+      } else {
+        cp_async_16(to + weight_offset<S>(base + w_row, w_col), src, bytes);
+      }
+      const int next = base + kRowsAtOnce;
+      if (bytes) src += kDown || next % 8 != 0 ? rows_down : next % 16 == 8 ? gate_to_up : up_to_gate;
+    }
+  };
+  // The elements of the group's tokens that belong to them.
+  auto issue_tokens = [&](uint32_t to) {
+    const bool whole = (step + 1) * S::kStep <= K;
+#pragma unroll
+    for (int i = 0; i < kTokenCopies; ++i) {
+      const int slot = (i * 32 + lane) / S::kTokenPieces, piece = (i * 32 + lane) % S::kTokenPieces;
       if (slot < live) {
-        const int token = r.token[at.a][at.group * kGroup + slot];
-        const int k = k0 + piece / S::kParts * 8;
-        const int bytes = k < K ? 16 : 0;
-        const void* src;
-        if constexpr (kDown) {
-          src = p.act + (static_cast<int64_t>(r.pair[at.a][token]) * (p.inter / 8) + (bytes ? k / 8 : 0)) * 2 +
-                piece % S::kParts;
-        } else {
-          src = p.x + static_cast<int64_t>(token) * p.hidden + (bytes ? k : 0);
-        }
-        cp_async_16(to + token_offset<S>(slot, piece), src, bytes);
+        const bool inside = whole || step * S::kStep + piece / S::kParts * 8 < K;
+        cp_async_16(to + token_offset<S>(slot, piece), inside ? t_src[i] : reinterpret_cast<const uint8_t*>(p.w),
+                    inside ? 16 : 0);
       }
     }
   };
-
-  // The warp's chunks of all its tiles as one sequence, of which `ahead` is the next to be issued.
-  Place ahead = {0, 0, 0};
-  int ahead_tile = my_chunks ? blockIdx.x : tiles, ahead_chunk = 0, filled = 0;
-  auto ahead_step = [&]() {  // seeks the place, returns the contraction step
-    const int c = warp + ahead_chunk * kWarps;
-    if (kDown) {
-      if (ahead_chunk == 0) ahead.a = 0;
-      ahead.seek(r, c);
-      return ahead.unit;
-    }
-    if (ahead_chunk == 0) ahead.seek(r, ahead_tile);
-    return c;
-  };
   auto advance = [&]() {
     filled = filled + 1 == S::kStages ? 0 : filled + 1;
-    if (++ahead_chunk >= my_chunks) { ahead_chunk = 0; if (ahead_tile < tiles) ahead_tile += gridDim.x; }
+    if (ahead_tile >= tiles) return;
+    if (++ahead_chunk >= my_chunks) {
+      ahead_chunk = 0;
+      ahead_tile += gridDim.x;
+      if (kDown) ahead.a = 0;
+      if (ahead_tile < tiles) locate();
+    } else if (kDown && warp + ahead_chunk * kWarps >= ahead.until) {
+      locate();
+    } else {
+      step += step_by;
+      const uint32_t bytes = static_cast<uint32_t>(step_by) * (S::kStep * 2);
+      w_src += bytes;
+#pragma unroll
+      for (int i = 0; i < kTokenCopies; ++i) t_src[i] += bytes * S::kParts;
+    }
   };
   auto issue_next = [&]() {
     if (ahead_tile < tiles) {
-      const int step = ahead_step();
-      const uint32_t to = ring + filled * S::kStageBytes;
-      issue_weights(ahead_tile, ahead, step, to);
-      issue_tokens(ahead, step, to);
+      issue_weights(ring + filled * S::kStageBytes);
+      issue_tokens(ring + filled * S::kStageBytes);
     }
     cp_async_commit();
     advance();
   };
+  if (ahead_tile < tiles) locate();
   if constexpr (kDown) {
     // Weights first, then, once kernel 1 is through, the activations that go with them.
     const int tile0 = ahead_tile;
     for (int s = 0; s < S::kStages - 1; ++s) {
-      if (ahead_tile < tiles) {
-        const int step = ahead_step();
-        issue_weights(ahead_tile, ahead, step, ring + filled * S::kStageBytes);
-      }
+      if (ahead_tile < tiles) issue_weights(ring + filled * S::kStageBytes);
       advance();
     }
-    ahead_tile = tile0; ahead_chunk = 0; filled = 0; ahead = {0, 0, 0};
+    ahead_tile = tile0; ahead_chunk = 0; filled = 0; ahead.a = 0;
+    if (ahead_tile < tiles) locate();
     pdl_wait();
     for (int s = 0; s < S::kStages - 1; ++s) {
-      if (ahead_tile < tiles) {
-        const int step = ahead_step();
-        issue_tokens(ahead, step, ring + filled * S::kStageBytes);
-      }
+      if (ahead_tile < tiles) issue_tokens(ring + filled * S::kStageBytes);
       cp_async_commit();
       advance();
     }
   } else {
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < S::kStages - 1; ++s) issue_next();
   }
 
-  int stage = 0, parity = 0;
-  Place here = {0, 0, 0};
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    float acc[S::kSets][kRT][kNT][4];
+  // ---- The computing side.  Columns of the products are the slots of a stage; what is left in slots
+  // without a token stays in columns that nobody reads.
+  // Matrix loads: lane l names row l % 8 of matrix l / 8.  Weights: rows 0..7 and 8..15 of 8 elements, then
+  // the same of the next 8.  Tokens: eight slots of 8 elements, four times in a row.
+  const int m_row = lane & 15, m_col = lane >> 4;
+  int stage = 0, parity = 0, here_live = 0;
+  Place here = {0, 0, 0, 0, 1};
+  float acc[S::kSets][kRT][kCT][4];
+  auto clear = [&]() {
 #pragma unroll
     for (int s = 0; s < S::kSets; ++s)
 #pragma unroll
       for (int m = 0; m < kRT; ++m)
 #pragma unroll
-        for (int n = 0; n < kNT; ++n)
+        for (int n = 0; n < kCT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[s][m][n][j] = 0.f;
-    if (kDown) here = {0, 0, 0}; else here.seek(r, tile);
+  };
+  auto look_up = [&](int at) {
+    here.seek(r, at);
+    here_live = min(r.count[here.a] - here.group * kGroup, kGroup);
+  };
+  // Element (row, token) of a warp's tile in kernel 2; rows shifted against bank conflicts.
+  auto sum_at = [&](int w, int row, int token) -> float& {
+    return s_sum[w * S::kSumFloats + row * S::kMaxT + (token ^ ((row & 7) << 2) % S::kMaxT)];
+  };
+  // Kernel 2, when the expert or the group changes: adds the columns to the tokens they belong to.
+  auto flush = [&]() {
+#pragma unroll
+    for (int n = 0; n < kCT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int slot = n * 8 + 2 * t + c;
+        if (slot < here_live) {
+          const int token = r.token[here.a][here.group * kGroup + slot];
+#pragma unroll
+          for (int m = 0; m < kRT; ++m) {
+            float lo = acc[0][m][n][c], hi = acc[0][m][n][c + 2];
+            if (S::kSets == 2) { lo += acc[S::kSets - 1][m][n][c]; hi += acc[S::kSets - 1][m][n][c + 2]; }
+            sum_at(warp, m * 16 + g, token) += lo;
+            sum_at(warp, m * 16 + g + 8, token) += hi;
+          }
+        }
+      }
+    clear();
+  };
+  // Products of one stage with the first kN column tiles.
+  auto multiply = [&](uint32_t at, auto tiles_of_8) {
+    constexpr int kN = decltype(tiles_of_8)::value;
+#pragma unroll
+    for (int kk = 0; kk < S::kStep / 32; ++kk) {
+      uint32_t a[2][kRT][4], b[kN][S::kParts][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < kRT; ++m)
+          ldmatrix_x4(a[h][m], at + weight_offset<S>(m * 16 + m_row, kk * 4 + h * 2 + m_col));
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int part = 0; part < S::kParts; ++part)
+          ldmatrix_x4(b[n][part], at + token_offset<S>(n * 8 + (lane & 7), (kk * 4 + (lane >> 3)) * S::kParts + part));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int part = 0; part < S::kParts; ++part)
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int m = 0; m < kRT; ++m)
+              Mma<__nv_bfloat16>::run(acc[h * (S::kSets - 1)][m][n], a[h][m], b[n][part][2 * h], b[n][part][2 * h + 1]);
+    }
+  };
+
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    clear();
+    if (kDown) { here = {0, 0, 0, 0, 1}; here_live = 0; } else look_up(tile);
 
     for (int i = 0; i < my_chunks; ++i) {
-      if (kDown) here.seek(r, warp + i * kWarps);
+      if (kDown && warp + i * kWarps >= here.until) {
+        flush();
+        look_up(warp + i * kWarps);
+      }
       issue_next();
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint32_t at = ring + stage * S::kStageBytes;
-      int slot[kNT];  // where the lane's token of each column tile stands in the stage; -1: a zero column
-      const uint32_t used = r.tiles[here.a][here.group];
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        const int rank = r.rank[here.a][n * 8 + g] - here.group * kGroup;
-        slot[n] = rank < kGroup ? rank : -1;
-      }
-#pragma unroll
-      for (int kk = 0; kk < S::kStep / 32; ++kk) {
-        uint32_t a0[kRT][4], a1[kRT][4];
-#pragma unroll
-        for (int m = 0; m < kRT; ++m) {
-          const uint4 lo = lds_16(at + weight_offset<S>(m * 16 + g, kk * 4 + t));
-          const uint4 hi = lds_16(at + weight_offset<S>(m * 16 + g + 8, kk * 4 + t));
-          a0[m][0] = lo.x; a0[m][1] = hi.x; a0[m][2] = lo.y; a0[m][3] = hi.y;
-          a1[m][0] = lo.z; a1[m][1] = hi.z; a1[m][2] = lo.w; a1[m][3] = hi.w;
-        }
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          if (kNT > 1 && !(used >> n & 1)) continue;
-#pragma unroll
-          for (int h = 0; h < S::kParts; ++h) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (slot[n] >= 0) b = lds_16(at + token_offset<S>(slot[n], (kk * 4 + t) * S::kParts + h));
-#pragma unroll
-            for (int m = 0; m < kRT; ++m) {
-              Mma<__nv_bfloat16>::run(acc[0][m][n], a0[m], b.x, b.y);
-              Mma<__nv_bfloat16>::run(acc[S::kSets - 1][m][n], a1[m], b.z, b.w);
-            }
-          }
-        }
-      }
+      if (kCT == 1 || here_live <= 8) multiply(at, std::integral_constant<int, 1>());
+      else multiply(at, std::integral_constant<int, kCT>());
       __syncwarp();  // the stage is refilled by a later iteration's copies
       stage = stage + 1 == S::kStages ? 0 : stage + 1;
     }
 
     // Add the warps up, in their order.
-    if (sizeof(s_sum) / sizeof(s_sum[0]) == 1) __syncthreads();  // with two buffers, one barrier per tile is enough
+    if constexpr (kDown) {
+      flush();
+      __syncthreads();
+      for (int i = threadIdx.x; i < S::kRows * S::kMaxT; i += kThreads) {
+        const int row = i % S::kRows, token = i / S::kRows;
+        float v = 0.f;
 #pragma unroll
-    for (int m = 0; m < kRT; ++m)
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        float4 v = make_float4(acc[0][m][n][0], acc[0][m][n][1], acc[0][m][n][2], acc[0][m][n][3]);
-        if (S::kSets == 2) {
-          v.x += acc[S::kSets - 1][m][n][0]; v.y += acc[S::kSets - 1][m][n][1];
-          v.z += acc[S::kSets - 1][m][n][2]; v.w += acc[S::kSets - 1][m][n][3];
+        for (int w = 0; w < kWarps; ++w) {
+          v += sum_at(w, row, token);
+          sum_at(w, row, token) = 0.f;
         }
-        s_sum[parity][warp][m * kNT + n][lane] = v;
+        if (token < p.tokens)
+          p.out[static_cast<int64_t>(token) * p.hidden + tile * S::kRows + row] = __float2bfloat16_rn(v);
       }
-    __syncthreads();
-    if (warp < kNT * kRT) {
-      float4 v = s_sum[parity][0][warp][lane];
+      __syncthreads();
+    } else {
+      // Two buffers in turn make one barrier per tile enough.
+      float4* sums = reinterpret_cast<float4*>(s_sum) + parity * kWarps * kRT * kCT * 32;
+      parity ^= 1;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 o = s_sum[parity][w][warp][lane];
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      const int m = warp / kNT, n = warp % kNT;
-      // Elements (row g, tokens 2 t, 2 t + 1) and (row g + 8, the same tokens) of row tile m.
-      const float top[2] = {v.x, v.y}, bottom[2] = {v.z, v.w};
+      for (int m = 0; m < kRT; ++m)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int token = n * 8 + 2 * t + c;
-        if constexpr (kDown) {
-          if (token < p.tokens) {
-            __nv_bfloat16* o = p.out + static_cast<int64_t>(token) * p.hidden + tile * S::kRows + m * 16 + g;
-            o[0] = __float2bfloat16_rn(top[c]);
-            o[8] = __float2bfloat16_rn(bottom[c]);
+        for (int n = 0; n < kCT; ++n) {
+          float4 v = make_float4(acc[0][m][n][0], acc[0][m][n][1], acc[0][m][n][2], acc[0][m][n][3]);
+          if (S::kSets == 2) {
+            v.x += acc[S::kSets - 1][m][n][0]; v.y += acc[S::kSets - 1][m][n][1];
+            v.z += acc[S::kSets - 1][m][n][2]; v.w += acc[S::kSets - 1][m][n][3];
           }
-        } else {
-          const int rank = r.rank[here.a][token];
-          if (rank >= 0 && rank / kGroup == here.group) {
-            const float value = r.weight[here.a][token] * (top[c] / (1.f + expf(-top[c])) * bottom[c]);
+          sums[(warp * kRT * kCT + m * kCT + n) * 32 + lane] = v;
+        }
+      __syncthreads();
+      if (warp < kRT * kCT) {
+        float4 v = sums[warp * 32 + lane];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+          const float4 o = sums[(w * kRT * kCT + warp) * 32 + lane];
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        const int m = warp / kCT, n = warp % kCT;
+        // Gate element g and up element g of row tile m, for slots 2 t and 2 t + 1.
+        const float gate[2] = {v.x, v.y}, up[2] = {v.z, v.w};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int slot = n * 8 + 2 * t + c, place = here.group * kGroup + slot;
+          if (slot < here_live) {
+            const float value = r.weight[here.a][place] * (gate[c] / (1.f + expf(-gate[c])) * up[c]);
             const __nv_bfloat16 high = __float2bfloat16_rn(value);
             const float rest = value - __bfloat162float(high);
             __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(
-                p.act + (static_cast<int64_t>(r.pair[here.a][token]) * (p.inter / 8) + here.unit * kRT + m) * 2);
+                p.act + (static_cast<int64_t>(r.pair[here.a][place]) * (p.inter / 8) + here.unit * kRT + m) * 2);
             o[g] = high;
             o[8 + g] = __float2bfloat16_rn(rest);
           }
         }
       }
     }
-    if (sizeof(s_sum) / sizeof(s_sum[0]) == 2) parity ^= 1;
   }
   cp_async_wait<0>();
 }
 
-template <int kNT, int kRT, bool kDown>
+template <int kCT, int kRT, bool kDown>
 int launch(const Params& p, int64_t tiles, cudaStream_t st) {
   const char* name = "moe_few_tokens";
-  const auto kernel = few_tokens_kernel<kNT, kRT, kDown>;
+  const auto kernel = few_tokens_kernel<kCT, kRT, kDown>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
   if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   const int64_t sms = sm_count();
@@ -413,16 +477,18 @@ int launch(const Params& p, int64_t tiles, cudaStream_t st) {
 }
 
 // 32-row tiles where there are more than 8 tokens and the sizes allow it.
-template <int kNT>
+template <int kCT>
 int launch(Params p, const void* w13, const void* w2, cudaStream_t st) {
+  constexpr int kRT = kCT;
   const int experts_hit = 2 * p.tokens < kExperts ? 2 * p.tokens : kExperts;
-  constexpr int kRT = kNT == 1 ? 1 : 2;
-  const bool wide_up = p.inter % (8 * kRT) == 0, wide_down = p.hidden % (16 * kRT) == 0;
-  p.w = static_cast<const __nv_bfloat16*>(w13);
   const int64_t up_tiles = static_cast<int64_t>(experts_hit) * p.inter / 8;
-  if (int rc = wide_up ? launch<kNT, kRT, false>(p, up_tiles / kRT, st) : launch<kNT, 1, false>(p, up_tiles, st)) return rc;
+  p.w = static_cast<const __nv_bfloat16*>(w13);
+  if (int rc = p.inter % (8 * kRT) == 0 ? launch<kCT, kRT, false>(p, up_tiles / kRT, st)
+                                        : launch<kCT, 1, false>(p, up_tiles, st))
+    return rc;
   p.w = static_cast<const __nv_bfloat16*>(w2);
-  return wide_down ? launch<kNT, kRT, true>(p, p.hidden / (16 * kRT), st) : launch<kNT, 1, true>(p, p.hidden / 16, st);
+  return p.hidden % (16 * kRT) == 0 ? launch<kCT, kRT, true>(p, p.hidden / (16 * kRT), st)
+                                    : launch<kCT, 1, true>(p, p.hidden / 16, st);
 }
 
 }  // namespace
@@ -472,7 +538,5 @@ extern "C" int b200moe_few_tokens(const void* hidden_states, const void* gating_
   p.logits_dtype = logits_dtype;
   p.renormalize = renormalize;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (num_tokens <= 8) return launch<1>(p, w13, w2, st);
-  if (num_tokens <= 16) return launch<2>(p, w13, w2, st);
-  return launch<4>(p, w13, w2, st);
+  return num_tokens <= 8 ? launch<1>(p, w13, w2, st) : launch<2>(p, w13, w2, st);
 }
