@@ -70,8 +70,8 @@ SIGNATURES = {
     "b200moe_paged_store_kvcache_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                 c_void_p, c_int, c_int64, c_int, c_int, c_int64, c_int64,
                                                 c_int64, c_int, c_void_p]),
-    "b200moe_paged_attn_fp8_num_splits": (c_int, [c_int, c_int, c_int64]),
-    "b200moe_paged_attn_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "b200moe_paged_attn_fp8_num_splits": (c_int, [c_int, c_int, c_int, c_int64]),
+    "b200moe_paged_attn_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200moe_paged_attn_varlen_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                               c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                               c_int64, c_int64, c_int, c_int, c_int64, c_float, c_int,

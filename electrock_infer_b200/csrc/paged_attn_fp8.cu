@@ -24,32 +24,46 @@
 // fp16 and bf16 values within 2^-38 of the row's largest), P is rounded to fp16 (2^-12 relative, below
 // the rounding of the output), all sums, maxima and the outputs are fp32.
 //
-// Four warps stream their own 32-token chunks through a three-stage ring of asynchronous 16-byte copies
+// Four warps stream their own 32-token chunks through rings of asynchronous 16-byte copies
 // (rows of 128 bytes, XOR-swizzled).  A page's K scale multiplies the scores; its V scale is the unit that
 // the accumulators are kept in, which is exchanged only where a warp comes to another page.  With
-// num_splits > 1 the context is cut into ranges for separate CTAs and a second kernel merges them.
+// num_splits > 1 the context is cut into ranges for separate CTAs: 2, 4 or 8 of them form a thread-block
+// cluster and merge through distributed shared memory where every CTA has an SM to itself; else they go
+// through a workspace and a second kernel.
+// (The tensor cores of sm_100a take codes directly only through tcgen05; m16n8k32 of codes is carried out as
+// conversions and products of fp16, and measured a tenth slower than converting here.)
 // Bound by HBM: 256 bytes per token and KV head.
+#include <cooperative_groups.h>
+
 #include "fp8_cache.cuh"
 #include "warp_mma.cuh"
 
 namespace b200moe {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kDim = kCodeHeadDim;
+constexpr int kTile = 16;                  // tokens of one product; a tile never crosses a page
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 16;                  // tokens of one product; a tile never crosses a page
 constexpr int kChunkTiles = 2;             // tiles per ring stage
 constexpr int kChunk = kTile * kChunkTiles;
-constexpr int kStages = 3;
 constexpr int kHalfBytes = kChunk * kDim;  // 4 KiB of K, as much of V
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kRingBytes = kWarps * kStages * kStageBytes;                    // 96 KiB
-constexpr int kScaleBytes = kWarps * kStages * 2 * kChunkTiles * sizeof(float);
-constexpr int kSmemBytes = kRingBytes + kScaleBytes;                          // two CTAs per SM
+// kNT = tiles of 8 query heads.  One tile: a two-stage ring and three CTAs per SM (measured 5 to 15 % faster
+// than three stages and two CTAs); two tiles need the registers of two CTAs per SM, whose rings then have
+// three stages.
+template <int kNT> struct Ring {
+  static constexpr int kStages = kNT == 1 ? 2 : 3;
+  static constexpr int kCtas = kNT == 1 ? 3 : 2;
+  static constexpr int kBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kSmemBytes = kBytes + kWarps * kStages * 2 * kChunkTiles * static_cast<int>(sizeof(float));
+};
+constexpr int kMaxCluster = 8;             // splits that merge through distributed shared memory
 constexpr int kMaxGroup = 16;
 constexpr int kMaxSplits = 64;
-constexpr int kMaxContext = 0x7fffffff - 2 * kChunk;  // so that rounding up to chunks stays in range
+constexpr int kMaxContext = 0x7fffffff - 4 * kTile;  // so that rounding up to chunks stays in range
 constexpr float kSlack = 8.f;              // in powers of two
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -82,9 +96,10 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int col) {
   return static_cast<uint32_t>(row * kDim + ((col ^ (row & 7)) << 4));
 }
 
-template <typename T, int kNT>  // kNT = tiles of 8 query heads
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, int kNT>
+__global__ void __launch_bounds__(kThreads, Ring<kNT>::kCtas)
 paged_attn_fp8_kernel(const Params p) {
+  constexpr int kStages = Ring<kNT>::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -94,9 +109,13 @@ paged_attn_fp8_kernel(const Params p) {
   pdl_wait();
   pdl_launch_dependents();
 
+  // The table row is on its way while the context length is being read.
+  const int32_t* table = p.block_table + seq * p.table_stride;
+  if (threadIdx.x * 32 < p.max_blocks) asm volatile("prefetch.global.L1 [%0];" ::"l"(table + threadIdx.x * 32));
   // A context never reaches past the pages the table row can name.
   const int ctx = static_cast<int>(min(static_cast<int64_t>(min(max(p.context_lens[seq], 0), kMaxContext)),
                                        static_cast<int64_t>(p.max_blocks) * p.block_size));
+  // (Ranges of one length for all sequences, so that shorter contexts take fewer CTAs, measured 5 to 20 % slower.)
   int per_split = (ctx - 1) / p.num_splits + 1;
   per_split = ((per_split - 1) / kChunk + 1) * kChunk;
   const int t_begin = static_cast<int>(min(static_cast<int64_t>(split) * per_split, static_cast<int64_t>(ctx)));
@@ -104,9 +123,8 @@ paged_attn_fp8_kernel(const Params p) {
   const int num_chunks = (t_end - t_begin + kChunk - 1) / kChunk;
 
   const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
-  float* scales = reinterpret_cast<float*>(smem + kRingBytes) + warp * kStages * 2 * kChunkTiles;
+  float* scales = reinterpret_cast<float*>(smem + Ring<kNT>::kBytes) + warp * kStages * 2 * kChunkTiles;
   const uint32_t scales_addr = smem_addr(scales);
-  const int32_t* table = p.block_table + seq * p.table_stride;
   const int64_t row_bytes = static_cast<int64_t>(p.kv_heads) * kDim;
 
   // What a lane copies of every tile: column `col` of rows `row`, row + 4, row + 8, row + 12.
@@ -158,7 +176,7 @@ paged_attn_fp8_kernel(const Params p) {
     cp_async_commit();
   };
 
-  // Warp w owns chunks w, w + 4, w + 8, ... of the CTA's range.
+  // Warp w owns chunks w, w + kWarps, w + 2 * kWarps, ... of the CTA's range.
   const int my_chunks = num_chunks > warp ? (num_chunks - warp + kWarps - 1) / kWarps : 0;
   auto chunk_index = [&](int i) { return i < my_chunks ? warp + i * kWarps : num_chunks; };
 #pragma unroll
@@ -355,9 +373,14 @@ paged_attn_fp8_kernel(const Params p) {
   cp_async_wait<0>();
   __syncthreads();
 
-  // Merge the four warps through shared memory (the ring is free now).
-  float* sm_o = reinterpret_cast<float*>(smem);          // [warps][kNT * 8][128]
-  float* sm_ml = sm_o + kWarps * kNT * 8 * kDim;         // [warps][kNT * 8][2]
+  // Merge the warps through shared memory (the ring is free now).  Columns are spread by two words in
+  // 16 and rows by 20 against bank conflicts.
+  constexpr int kHeads = kNT * 8, kPitch = kDim + 20;
+  float* sm_o = reinterpret_cast<float*>(smem);              // [warps][kHeads][kPitch]
+  float* sm_ml = sm_o + kWarps * kHeads * kPitch;            // [warps][kHeads][2]: maximum, sum
+  float* sm_f = sm_ml + kWarps * kHeads * 2;                 // [kHeads][warps]: the warps' weights
+  float* sm_total = sm_f + kHeads * kWarps;                  // [kHeads][2]: the CTA's maximum and sum
+  float* sm_acc = sm_total + kHeads * 2;                     // [kHeads][128]: the CTA's output
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
 #pragma unroll
@@ -366,8 +389,8 @@ paged_attn_fp8_kernel(const Params p) {
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int row = warp * kNT * 8 + n * 8 + 2 * t + c;
-      float* wo = sm_o + row * kDim + g * 16;
+      const int row = warp * kHeads + n * 8 + 2 * t + c;
+      float* wo = sm_o + row * kPitch + g * 18;
 #pragma unroll
       for (int m = 0; m < kDim / 16; ++m)
         *reinterpret_cast<float2*>(wo + 2 * m) = make_float2(o[n][m][c] * unit, o[n][m][c + 2] * unit);
@@ -378,34 +401,76 @@ paged_attn_fp8_kernel(const Params p) {
     }
   }
   __syncthreads();
-  // Thread d owns output dimension d for every head of the group.
-  const int d = threadIdx.x;
-  for (int r = 0; r < p.group; ++r) {
-    float mw[kWarps], top = -INFINITY;
+  if (threadIdx.x < kHeads) {
+    float2 ml[kWarps];
+    float top = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      mw[w] = sm_ml[(w * kNT * 8 + r) * 2];
-      top = fmaxf(top, mw[w]);
+      ml[w] = *reinterpret_cast<const float2*>(sm_ml + (w * kHeads + threadIdx.x) * 2);
+      top = fmaxf(top, ml[w].x);
     }
-    float l = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float lw = sm_ml[(w * kNT * 8 + r) * 2 + 1];
-      const float f = lw == 0.f ? 0.f : exp2f(mw[w] - top);  // a warp without tokens has sum 0
-      l += f * lw;
-      acc += f * sm_o[(w * kNT * 8 + r) * kDim + d];
+      const float f = ml[w].y == 0.f ? 0.f : exp2f(ml[w].x - top);  // a warp without tokens has sum 0
+      sm_f[threadIdx.x * kWarps + w] = f;
+      l += f * ml[w].y;
     }
-    const int64_t head = static_cast<int64_t>(seq) * p.q_heads + static_cast<int64_t>(kvh) * p.group + r;
+    sm_total[threadIdx.x * 2] = top;
+    sm_total[threadIdx.x * 2 + 1] = l;
+  }
+  __syncthreads();
+  const int64_t head0 = static_cast<int64_t>(seq) * p.q_heads + static_cast<int64_t>(kvh) * p.group;
+  const bool in_cluster = p.num_splits > 1 && p.ws_o == nullptr;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < p.group * kDim; i += kThreads) {
+    const int r = i / kDim, d = i % kDim;
+    const float* wo = sm_o + r * kPitch + d + 2 * (d / 16);
+    float acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) acc += sm_f[r * kWarps + w] * wo[w * kHeads * kPitch];
     if (p.num_splits == 1) {
       // An empty context gives zeros (the reference divides 0 by 0 there).
-      static_cast<T*>(p.out)[head * kDim + d] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
+      const float l = sm_total[r * 2 + 1];
+      static_cast<T*>(p.out)[head0 * kDim + i] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
+    } else if (in_cluster) {
+      sm_acc[i] = acc;
     } else {
-      p.ws_o[(head * p.num_splits + split) * kDim + d] = acc;
-      if (d == 0) {
-        p.ws_ml[(head * p.num_splits + split) * 2] = top;
-        p.ws_ml[(head * p.num_splits + split) * 2 + 1] = l;
-      }
+      p.ws_o[((head0 + r) * p.num_splits + split) * kDim + d] = acc;
+      if (d < 2) p.ws_ml[((head0 + r) * p.num_splits + split) * 2 + d] = sm_total[r * 2 + d];
     }
+  }
+  if (in_cluster) {
+    // The splits of this (sequence, KV head) are the CTAs of one cluster: each finishes its share of the
+    // outputs from all of them.
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int outputs = p.group * kDim, share = (outputs + p.num_splits - 1) / p.num_splits;
+    const int end = min((split + 1) * share, outputs);
+    for (int i = split * share + threadIdx.x; i < end; i += kThreads) {
+      const int r = i / kDim;
+      float2 ml[kMaxCluster];
+      float v[kMaxCluster], top = -INFINITY, l = 0.f, acc = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        if (s < p.num_splits) {
+          ml[s] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sm_total, s) + r * 2);
+          v[s] = cluster.map_shared_rank(sm_acc, s)[i];
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s)
+        if (s < p.num_splits) top = fmaxf(top, ml[s].x);
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        if (s < p.num_splits) {
+          const float f = ml[s].y == 0.f ? 0.f : exp2f(ml[s].x - top);
+          l += f * ml[s].y;
+          acc += f * v[s];
+        }
+      }
+      static_cast<T*>(p.out)[head0 * kDim + i] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
+    }
+    cluster.sync();  // no CTA leaves while another may still read its part
   }
 }
 
@@ -458,16 +523,38 @@ paged_attn_fp8_merge_kernel(const float* __restrict__ ws_o, const float* __restr
   out[head * kDim + d] = Mma<T>::from_float(l == 0.f ? 0.f : acc / l);
 }
 
+// Whether the splits of `pairs` (sequence, KV head) pairs merge inside the kernel.  Clusters start and end
+// together, which costs more than the second kernel once CTAs have to share SMs (128 sequences x 8 heads x
+// 8192 tokens in 8 splits: 338 us as clusters).
+inline bool merges_in_cluster(int64_t pairs, int num_splits) {
+  return (num_splits == 2 || num_splits == 4 || num_splits == kMaxCluster) && pairs * num_splits <= sm_count();
+}
+
 template <typename T, int kNT>
 int launch(const Params& p, int batch, cudaStream_t st) {
+  const char* name = "paged_attn_varlen_fp8";
+  const auto kernel = paged_attn_fp8_kernel<T, kNT>;
+  const bool in_cluster = merges_in_cluster(static_cast<int64_t>(batch) * p.kv_heads, p.num_splits);
   // Per device and per function; cheap enough to repeat on every call.
-  const cudaError_t e = cudaFuncSetAttribute(
-      paged_attn_fp8_kernel<T, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "paged_attn_varlen_fp8: %s", cudaGetErrorString(e));
-  const int64_t ctas = static_cast<int64_t>(batch) * p.kv_heads * p.num_splits;
-  launch_pdl(paged_attn_fp8_kernel<T, kNT>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmemBytes, st, p);
-  if (int rc = check_launch("paged_attn_varlen_fp8")) return rc;
-  if (p.num_splits > 1) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kNT>::kSmemBytes);
+  if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(batch) * p.kv_heads * p.num_splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Ring<kNT>::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.num_splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = in_cluster ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, p);
+  if (int rc = check_launch(name)) return rc;
+  if (p.num_splits > 1 && !in_cluster) {
     launch_pdl(paged_attn_fp8_merge_kernel<T>, dim3(static_cast<unsigned>(batch * p.q_heads)), dim3(kDim), 0, st,
                static_cast<const float*>(p.ws_o), static_cast<const float*>(p.ws_ml), static_cast<T*>(p.out),
                p.num_splits);
@@ -479,21 +566,41 @@ int launch(const Params& p, int batch, cudaStream_t st) {
 }  // namespace
 }  // namespace b200moe
 
-extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int kv_heads, int64_t max_context) {
+extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_heads, int64_t max_context) {
   using namespace b200moe;
-  if (batch < 1 || kv_heads < 1 || max_context < 1) return 1;
-  const int64_t ctas = static_cast<int64_t>(batch) * kv_heads;
-  const int64_t want = ceil_div64(6ll * sm_count(), ctas);
-  const int64_t by_length = max_context / 512 > 0 ? max_context / 512 : 1;
-  int64_t s = want < by_length ? want : by_length;
-  if (s < 1) s = 1;
-  if (s > kMaxSplits) s = kMaxSplits;
-  return static_cast<int>(s);
+  if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || max_context < 1) return 1;
+  // Estimated time of each number of splits, from measurements with 1 to 128 sequences of 100 to 60000
+  // tokens (1 x 8 heads x 700 tokens: 8.5 us unsplit, 5.5 us in 8 splits; 16 x 8 x 8192: 66 us unsplit, 43 us
+  // in 3; 128 x 8 x 8192: 283 us unsplit, 256 us in 3; 16 x 8 x 1024: 10.9 us unsplit, 11.7 us in 3).  In ns:
+  // a CTA takes 7.4 a token when it has an SM to itself, 11.6 and 13.8 with one and two others beside it
+  // (10.5 and 14.7 with two head tiles); beyond one wave the GPU is filled evenly, but for a last wave of half
+  // a CTA's time and 1.2 us per CTA and wave; merging takes 2.4 us in a cluster, else 3.2 us and 80 ns a split.
+  const bool wide = q_heads / kv_heads > 8;
+  const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, sms = sm_count();
+  const int64_t slots = sms * (wide ? Ring<2>::kCtas : Ring<1>::kCtas);
+  const double by_share[3] = {wide ? 10.5 : 7.4, wide ? 14.7 : 11.6, 13.8};
+  int best = 1;
+  double best_cost = 0;
+  for (int s = 1; s <= kMaxSplits; ++s) {
+    if (s > 1 && max_context < static_cast<int64_t>(s - 1) * kChunk) break;
+    const int64_t ctas = pairs * s;
+    const double tokens = static_cast<double>(max_context) / s;
+    const int64_t per_sm = ceil_div64(ctas < slots ? ctas : slots, sms);
+    double cost = tokens * by_share[per_sm - 1];
+    if (ctas > slots) cost *= static_cast<double>(ctas) / slots + 0.5;
+    if (ctas > slots) cost += 1200.0 * ctas / slots;
+    if (s > 1) cost += merges_in_cluster(pairs, s) ? 2400.0 : 3200.0 + 80.0 * s;
+    if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
+  }
+  return best;
 }
 
-extern "C" size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int num_splits) {
-  if (batch < 1 || q_heads < 1 || num_splits <= 1) return 0;
-  return static_cast<size_t>(batch) * q_heads * num_splits * (b200moe::kDim + 2) * sizeof(float);
+extern "C" size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int kv_heads, int num_splits) {
+  using namespace b200moe;
+  if (batch < 1 || q_heads < 1 || kv_heads < 1 || num_splits <= 1 ||
+      merges_in_cluster(static_cast<int64_t>(batch) * kv_heads, num_splits))
+    return 0;
+  return static_cast<size_t>(batch) * q_heads * num_splits * (kDim + 2) * sizeof(float);
 }
 
 extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache, const void* v_cache,
@@ -543,8 +650,8 @@ extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache,
   p.max_blocks = max_blocks_per_seq; p.num_splits = num_splits; p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * kLog2e;
   p.by_block = FastDiv::by(static_cast<uint32_t>(block_size));
-  if (num_splits > 1) {
-    const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, num_splits);
+  const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, kv_heads, num_splits);
+  if (need > 0) {
     if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
       return fail(B200MOE_ERR_WORKSPACE, "%s: num_splits=%d needs a 16-byte aligned workspace of "
                   "%zu bytes, got %zu", name, num_splits, need, workspace_bytes);

@@ -232,11 +232,12 @@ Tensor paged_attn_varlen_fp8(const Args& a) {
   if (splits <= 0) {
     int64_t longest = width * c.block_size;
     if (max_len > 0 && max_len < longest) longest = max_len;
-    splits = b200moe_paged_attn_fp8_num_splits(static_cast<int>(batch), static_cast<int>(c.heads), longest);
+    splits = b200moe_paged_attn_fp8_num_splits(static_cast<int>(batch), static_cast<int>(heads),
+                                               static_cast<int>(c.heads), longest);
   }
   Tensor out = at::empty({batch, heads, c.dim}, q.options());
   const size_t bytes = b200moe_paged_attn_fp8_workspace_bytes(static_cast<int>(batch), static_cast<int>(heads),
-                                                              static_cast<int>(splits));
+                                                              static_cast<int>(c.heads), static_cast<int>(splits));
   Tensor ws;
   if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
   check_status(b200moe_paged_attn_varlen_fp8(

@@ -444,15 +444,17 @@ int b200moe_paged_schedule(const int32_t* context_lens, const int32_t* new_lens,
  * b200moe_paged_attn_varlen_fp8 is b200moe_paged_attn_varlen over such caches; q rows are q_row_stride
  * elements apart (a multiple of 8), table rows table_row_stride.  Scores, softmax statistics and sums
  * are fp32, the probabilities are rounded to fp16 for the product with V.  A NaN in a context gives NaN;
- * codes past a context may be anything.
+ * codes past a context may be anything.  num_splits is 1 to 64 (b200moe_paged_attn_fp8_num_splits suggests
+ * a value); above 1 it may need a workspace of b200moe_paged_attn_fp8_workspace_bytes bytes, which is 0
+ * where the splits merge inside the kernel.  Both functions ask for the current device's SM count.
  */
 int b200moe_paged_store_kvcache_fp8(const void* key, const void* value, void* k_cache, void* v_cache,
                                     float* k_scale, float* v_scale, const int32_t* slot_mapping,
                                     int dtype, int64_t num_tokens, int num_kv_heads, int head_dim,
                                     int64_t key_row_stride, int64_t value_row_stride,
                                     int64_t num_blocks, int block_size, b200moe_stream_t stream);
-int b200moe_paged_attn_fp8_num_splits(int batch, int kv_heads, int64_t max_context);
-size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int num_splits);
+int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_heads, int64_t max_context);
+size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int kv_heads, int num_splits);
 int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache, const void* v_cache,
                                   const float* k_scale, const float* v_scale, void* out,
                                   const int32_t* block_table, const int32_t* context_lens, int dtype,

@@ -57,16 +57,19 @@ def test_attention_arguments():
     assert call(heads=34, qs=34 * 128) == -7
     assert call(q=None) == -3 and call(scale=None) == -3
     assert call(qs=1028) == -5 and call(q=ctypes.c_void_p(264)) == -5
-    need = lib.b200moe_paged_attn_fp8_workspace_bytes(2, 8, 3)
-    assert need > 0 and lib.b200moe_paged_attn_fp8_workspace_bytes(2, 8, 1) == 0
+    need = lib.b200moe_paged_attn_fp8_workspace_bytes(2, 8, 2, 3)
+    assert need > 0 and lib.b200moe_paged_attn_fp8_workspace_bytes(2, 8, 2, 1) == 0
+    # Two, four and eight splits of few sequences merge without one.
+    assert lib.b200moe_paged_attn_fp8_workspace_bytes(2, 8, 2, 8) == 0
+    assert lib.b200moe_paged_attn_fp8_workspace_bytes(200, 8, 2, 8) > 0
     assert call(splits=3, ws=PTR, ws_bytes=need - 1) == -4 and call(splits=3) == -4
     assert call(batch=0) == 0
 
 
 @pytest.mark.parametrize("batch,heads,longest", [(1, 1, 1), (1, 8, 700), (4, 1, 60001), (128, 8, 8192), (4000, 8, 10 ** 6), (1, 1, 2 ** 31 - 1)])
 def test_split_counts_are_in_range(batch, heads, longest):
-    s = _lib.load().b200moe_paged_attn_fp8_num_splits(batch, heads, longest)
-    assert 1 <= s <= 64
+    for group in (1, 4, 16):
+        assert 1 <= _lib.load().b200moe_paged_attn_fp8_num_splits(batch, heads * group, heads, longest) <= 64
 
 
 def test_ops_refuse_cpu_tensors():

@@ -232,6 +232,9 @@ def check_attn(c, got):
     (8, 8, 16, [33, 200, 1], 1),                               # no sharing
     (8, 1, 16, [129, 64, 640], 2),
     (12, 4, 48, [100, 47, 48, 49], 2),                         # groups of 3
+    (12, 4, 48, [300, 47, 1, 0, 2000], 4),
+    (10, 2, 32, [900, 1, 0, 64, 333], 8),
+    (16, 1, 64, [2048, 1, 0, 777], 8),
     (14, 2, 32, [5, 95], 1),                                   # groups of 7
     (9, 1, 64, [130, 63], 3),                                  # groups of 9: two head tiles
     (16, 1, 64, [2048, 1], 7),
@@ -299,6 +302,14 @@ def test_attention_passes_a_nan_of_the_context_on():
         assert torch.isnan(got[0, 4:]).all() and torch.isfinite(got[0, :4]).all() and torch.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("max_len", [1, 100, 999, 10 ** 9])
+@pytest.mark.parametrize("splits", [2, 5, 8, 37])
+def test_attention_with_any_idea_of_the_longest_context(max_len, splits):
+    """Contexts longer than max_seqlen_k are still attended to in full."""
+    c = attn_case([999, 30, 0, 512], 8, 2, 16, torch.float16, seed=4)
+    check_attn(c, attend(c, splits, max_len=max_len))
+
+
 def test_attention_lengths_beyond_the_table_are_cut():
     c = attn_case([64, 60], 4, 1, 32, torch.bfloat16, seed=2)
     want = attend({**c, "lens": torch.tensor([64, 64], dtype=torch.int32)}, 1)
@@ -361,5 +372,5 @@ def test_attention_refusals():
     rc = _lib.load().b200moe_paged_attn_varlen_fp8(
         d["q"].data_ptr(), d["k_cache"].data_ptr(), d["v_cache"].data_ptr(), d["k_scale"].data_ptr(), d["v_scale"].data_ptr(),
         d["q"].data_ptr(), d["table"].data_ptr(), d["lens"].data_ptr(), _lib.BF16, 2, 32, 8, 128, 32 * 128, d["k_cache"].size(0),
-        32, 1, 1, 0.1, 4, None, 0, torch.cuda.current_stream().cuda_stream)
-    assert rc == -4  # no workspace for num_splits = 4
+        32, 1, 1, 0.1, 5, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == -4  # no workspace for num_splits = 5
