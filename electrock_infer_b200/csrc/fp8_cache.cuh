@@ -37,9 +37,14 @@ __device__ __forceinline__ void codes_to_half2(uint32_t codes, uint32_t& low, ui
       : "r"(codes));
 }
 
-// Two fp32 values -> two codes, round to nearest even, too large values to the largest code.
-__device__ __forceinline__ uint32_t to_codes2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+// Four fp32 values -> four codes, round to nearest even, too large values to the largest code.
+__device__ __forceinline__ uint32_t to_codes4(float x0, float x1, float x2, float x3) {
+  uint32_t codes;
+  asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+      "mov.b32 %0, {l, h};\n\t}"
+      : "=r"(codes)
+      : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+  return codes;
 }
 
 // Four codes multiplied by `ratio` and rounded again.
@@ -48,7 +53,7 @@ __device__ __forceinline__ uint32_t rescale_codes4(uint32_t codes, float ratio) 
   codes_to_half2(codes, a, b);
   const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
   const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  return to_codes2(fa.x * ratio, fa.y * ratio) | (to_codes2(fb.x * ratio, fb.y * ratio) << 16);
+  return to_codes4(fa.x * ratio, fa.y * ratio, fb.x * ratio, fb.y * ratio);
 }
 
 }  // namespace b200moe

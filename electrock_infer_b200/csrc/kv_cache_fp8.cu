@@ -16,8 +16,8 @@
 //
 // The reference has no 8-bit cache; its store (src/store_kv_cache.hip:12-63) copies.  This one has to
 // know a run's largest value before it can write the first code, so the rows of a run are held in
-// registers between the two: short runs (decode: one token) by one warp, longer ones by the whole CTA,
-// 64 KB of 16-bit rows in flight.  A run that does not fit is read a second time (from L2).  Bound by HBM
+// registers between the two: short runs (decode: one token) by one warp, longer ones by the whole CTA.  A run
+// that does not fit is read a second time (from L2).  Bound by HBM
 // for prompts (16-bit rows in, 8-bit codes out: 3 bytes an element) and by latency for decode steps (slot ->
 // rows and old scale -> codes).
 #include "fp8_cache.cuh"
@@ -28,8 +28,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxSegment = 256;   // tokens whose runs one CTA may own
-constexpr int kWarpRows = 16;      // rows that one warp holds
-
+// 16-byte pieces of a run that a thread holds: 16 rows of 16-bit elements for a warp, 128 for the CTA.
+// Twice as many leave room for two CTAs per SM instead of three: 37 prompts of 26-53 tokens 9.3 us instead
+// of 7.0, 16 prompts of 512-1024 tokens 27.2 us instead of 27.5.
+constexpr int kPieces = 8;
 
 struct Side {  // keys or values
   const uint8_t* src;
@@ -208,8 +210,7 @@ __device__ void store_run(const Params& p, const Side& side, int head, int64_t f
       uint32_t codes[Row<T>::kElems / 4];
 #pragma unroll
       for (int j = 0; j < Row<T>::kElems / 4; ++j)
-        codes[j] = to_codes2(x[4 * j] * inv, x[4 * j + 1] * inv) |
-                   (to_codes2(x[4 * j + 2] * inv, x[4 * j + 3] * inv) << 16);
+        codes[j] = to_codes4(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
       uint8_t* dst = cache + slot[u] * row_bytes + col * Row<T>::kElems;
       if constexpr (Row<T>::kElems == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
       else *reinterpret_cast<uint32_t*>(dst) = codes[0];
@@ -218,7 +219,7 @@ __device__ void store_run(const Params& p, const Side& side, int head, int64_t f
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
 paged_store_fp8_kernel(const Params p) {
   __shared__ int s_begin[kMaxSegment], s_begin_page[kMaxSegment], s_page[kMaxSegment], s_long[kMaxSegment];
   __shared__ int s_num_begin, s_num_long, s_at;
@@ -284,8 +285,7 @@ paged_store_fp8_kernel(const Params p) {
       if (lane == 0) s_long[atomicAdd(&s_num_long, 1)] = k;
       continue;
     }
-    store_run<T, 1, kWarpRows * kCodeHeadDim / Row<T>::kElems / 32>(p, side, head, i, __ffs(out) - 1, run_page,
-                                                                    s_red);
+    store_run<T, 1, kPieces>(p, side, head, i, __ffs(out) - 1, run_page, s_red);
   }
   __syncthreads();
   for (int k = 0; k < s_num_long; ++k) {
@@ -304,7 +304,7 @@ paged_store_fp8_kernel(const Params p) {
       len += s_at;
       if (s_at < kThreads) break;
     }
-    store_run<T, kWarps, 16>(p, side, head, i, len, run_page, s_red);
+    store_run<T, kWarps, kPieces>(p, side, head, i, len, run_page, s_red);
   }
 }
 
