@@ -78,6 +78,10 @@ class FusedMoE(nn.Module):
         self.w13_weight.weight_loader = self.weight_loader
         self.w2_weight.weight_loader = self.weight_loader
 
+    def takes_few_tokens(self, num_tokens: int) -> bool:
+        """Whether a batch of this size takes the two-kernel path."""
+        return 0 < num_tokens <= self.few_token_limit
+
     def peer_reduce_for(self, hidden_states: torch.Tensor):
         """The ``TensorParallelReduce`` to hand to ``fused_experts`` for this batch, or None when
         the sum (if any) is an NCCL all-reduce.  Every rank sees the same token count, so every
@@ -85,7 +89,7 @@ class FusedMoE(nn.Module):
         if not (self.reduce_results and self.tp_size > 1) or self.tp_exchange == "nccl":
             return None
         num_tokens, hidden = hidden_states.shape
-        if num_tokens <= self.few_token_limit:
+        if self.takes_few_tokens(num_tokens):
             return None
         applies = (hidden_states.is_cuda and self.top_k == 2 and self.tp_size <= 8
                    and self.tp_size == dist.get_world_size() and dist.get_backend() == "nccl"
@@ -113,11 +117,11 @@ class FusedMoE(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         tp_reduce = self.peer_reduce_for(hidden_states)
+        few = {"few_tokens": True} if self.takes_few_tokens(hidden_states.size(0)) else {}
         final_hidden_states = fused_experts(
             hidden_states=hidden_states, w1=self.w13_weight, w2=self.w2_weight,
             gating_output=router_logits, topk=self.top_k, renormalize=self.renormalize,
-            inplace=True, activation="silu", tp_reduce=tp_reduce,
-            few_tokens=hidden_states.size(0) <= self.few_token_limit)
+            inplace=True, activation="silu", tp_reduce=tp_reduce, **few)
         if self.reduce_results and self.tp_size > 1 and tp_reduce is None:
             with _timed("all_reduce:result"):
                 dist.all_reduce(final_hidden_states)
@@ -181,7 +185,7 @@ class MixtralMoE(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         orig_shape = hidden_states.shape
         hidden_states = hidden_states.view(-1, self.hidden_size)
-        if self.fuse_gate and hidden_states.size(0) > self.experts.few_token_limit:
+        if self.fuse_gate and not self.experts.takes_few_tokens(hidden_states.size(0)):
             tp_reduce = self.experts.peer_reduce_for(hidden_states)
             out = fused_experts(hidden_states, self.experts.w13_weight, self.experts.w2_weight, None,
                                 self.experts.top_k, renormalize=True, inplace=True,

@@ -121,7 +121,9 @@ def test_few_token_layer_arguments():
             FusedMoE(8, 2, 64, 256, tp_size=1, **bad)
     with pytest.raises(ValueError):
         FusedMoE(4, 2, 64, 256, tp_size=1, few_token_limit=4)
-    assert FusedMoE(8, 2, 64, 256, tp_size=1).few_token_limit == 0
+    plain, few = FusedMoE(8, 2, 64, 256, tp_size=1), FusedMoE(8, 2, 64, 256, tp_size=1, few_token_limit=4)
+    assert [plain.takes_few_tokens(n) for n in (0, 1, 32)] == [False] * 3
+    assert [few.takes_few_tokens(n) for n in (0, 1, 4, 5)] == [False, True, True, False]
     with pytest.raises(RuntimeError, match="CUDA"):
         fused_experts(torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(8, 512, 256, dtype=torch.bfloat16),
                       torch.zeros(8, 256, 256, dtype=torch.bfloat16), torch.zeros(4, 8), 2, few_tokens=True)
