@@ -12,7 +12,8 @@
 // columns; a tile is 16 or 32 weight rows with the whole contraction, split over the eight warps of a CTA.
 // Each warp streams 4 KiB of weights per step, with the tokens' elements that belong to them, through a ring of
 // its own (asynchronous 16-byte copies, 192 KiB an SM), never waiting for another warp except to add up a
-// finished tile.  Tiles are dealt round-robin; that some CTAs get one more does not cost much,
+// finished tile (kernel 1 with a short contraction: each warp has its own tiles; kernel 2 with few tiles: a
+// thread-block cluster shares one).  Tiles are dealt round-robin; that some CTAs get one more does not cost much,
 // because an SM alone can draw well over 1/148 of the HBM rate.
 //
 // * Fragments come from matrix loads, whose registers are the products' operands as they are (16-byte
@@ -30,6 +31,7 @@
 //   waits for kernel 1.
 //
 // The reference runs the same batch through its general path (layers/moe/fused_moe.py:170-293).
+#include <cooperative_groups.h>
 #include <type_traits>
 
 #include "warp_mma.cuh"
@@ -37,7 +39,10 @@
 namespace b200moe {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kExperts = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxTokens = 32;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
@@ -52,6 +57,7 @@ struct Params {
   uint4* act;              // [2 * tokens][inter / 8][2]: eight high parts, eight low parts
   __nv_bfloat16* out;
   int tokens, hidden, inter, logits_dtype, renormalize;
+  int cluster;  // CTAs that share the contraction of a tile of kernel 2
 };
 
 // Experts that were hit, in ascending order, and their tokens.
@@ -126,24 +132,36 @@ __device__ void route(const Params& p, Routing& r, int units) {
   }
 }
 
-// A warp's way through the sequence of (active expert, unit, group of tokens): units are tiles of kernel 1
-// and contraction steps of kernel 2, the groups of one unit follow one another.
+// A warp's way through the sequence of (active expert, unit, group of tokens).  Kernel 1: units are tiles, and
+// the groups of one tile follow one another, so that its weights come from L2 the second time.  Kernel 2: units
+// are contraction steps, and the groups go through all of them one after the other, so that the columns
+// change seldom (an expert's rows of a tile stay in L2).
+template <bool kDown>
 struct Place {
-  int a, until, unit, group, groups;
+  int a, until, unit, group;  // `until`: end of the part of the sequence with the same expert and (kernel 2) group
   // Moves forward to position `at` of the sequence.
-  __device__ __forceinline__ void seek(const Routing& r, int at) {
+  __device__ __forceinline__ void seek(const Routing& r, int at, int units) {
     while (at >= r.begin[a + 1]) ++a;
-    until = r.begin[a + 1];
-    groups = r.count[a] > kGroup ? 2 : 1;
     const int rest = at - r.begin[a];
-    unit = groups == 2 ? rest >> 1 : rest;
-    group = groups == 2 ? rest & 1 : 0;
+    const bool two = r.count[a] > kGroup;
+    if (kDown) {
+      group = two && rest >= units ? 1 : 0;
+      unit = rest - group * units;
+      until = r.begin[a] + (group + 1) * units;
+    } else {
+      unit = two ? rest >> 1 : rest;
+      group = two ? rest & 1 : 0;
+      until = r.begin[a + 1];
+    }
   }
 };
 
 // kCT = tiles of 8 tokens that a stage has room for, kRT = tiles of 16 weight rows.
-template <int kCT, int kRT, bool kDown>
+// kAlone (kernel 1): a warp takes whole tiles by itself instead of an eighth of every tile.
+template <int kCT_, int kRT_, bool kDown_, bool kAlone_>
 struct Shape {
+  static constexpr int kCT = kCT_, kRT = kRT_;
+  static constexpr bool kDown = kDown_, kAlone = kAlone_;
   static constexpr int kStep = 128 / kRT;                      // contraction elements of a stage
   static constexpr int kPieces = kStep / 8;                    // 16-byte pieces of a weight row
   static constexpr int kParts = kDown ? 2 : 1;                 // numbers that an element is the sum of
@@ -155,7 +173,7 @@ struct Shape {
   static constexpr int kSets = kCT * kRT == 1 ? 2 : 1;         // accumulator sets, against dependent products
   static constexpr int kMaxT = kCT == 1 ? 8 : kMaxTokens;      // tokens of the batch
   // What the warps add up through: kernel 1 two buffers of accumulators, kernel 2 a tile per warp.
-  static constexpr int kSumFloats = kDown ? kRows * kMaxT : 2 * kRT * kCT * 32 * 4;
+  static constexpr int kSumFloats = kDown ? kRows * kMaxT : kAlone ? 4 : 2 * kRT * kCT * 32 * 4;
   static_assert(kStages >= 2, "the ring is too small");
 };
 
@@ -168,10 +186,11 @@ template <typename S> __device__ __forceinline__ uint32_t token_offset(int slot,
   return static_cast<uint32_t>(kWeightBytes + (slot * S::kTokenPieces + (piece ^ (slot & 7))) * 16);
 }
 
-template <int kCT, int kRT, bool kDown>
+template <typename S>
 __global__ void __launch_bounds__(kThreads, 1)
 few_tokens_kernel(const Params p) {
-  using S = Shape<kCT, kRT, kDown>;
+  constexpr int kCT = S::kCT, kRT = S::kRT;
+  constexpr bool kDown = S::kDown;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Routing r;
   __shared__ __align__(16) float s_sum[kWarps * S::kSumFloats];
@@ -191,7 +210,19 @@ few_tokens_kernel(const Params p) {
 
   const int chunks = kDown ? r.begin[r.num_active] : steps;                    // of one tile
   const int tiles = kDown ? expert_tiles : r.begin[r.num_active];
-  const int my_chunks = chunks > warp ? (chunks - warp + kWarps - 1) / kWarps : 0;  // of one tile
+  const int units = kDown ? steps : expert_tiles;
+  // The warp's chunks of a tile: every eighth (kernel 1; kernel 2: of those of the cluster that works on the tile,
+  // side by side for the sake of DRAM pages), all (kernel 1, alone), or, where an expert has too few for that, a
+  // range, so that the columns do not change all the time.
+  const int shares = kDown ? p.cluster * kWarps : S::kAlone ? 1 : kWarps;
+  const int share = kDown ? static_cast<int>(blockIdx.x % p.cluster) * kWarps + warp : S::kAlone ? 0 : warp;
+  const bool range = kDown && steps < 8 * shares;
+  const int next_chunk = range ? 1 : shares;
+  const int chunk0 = range ? static_cast<int>(static_cast<int64_t>(chunks) * share / shares) : share;
+  const int my_chunks = range ? static_cast<int>(static_cast<int64_t>(chunks) * (share + 1) / shares) - chunk0
+                      : chunks > share ? (chunks - share + shares - 1) / shares : 0;
+  const int tile0 = kDown ? blockIdx.x / p.cluster : S::kAlone ? warp * gridDim.x + blockIdx.x : blockIdx.x;
+  const int tile_step = kDown ? gridDim.x / p.cluster : S::kAlone ? gridDim.x * kWarps : gridDim.x;
   const uint32_t ring = smem_addr(smem) + warp * S::kStages * S::kStageBytes;
   const int64_t row_bytes = static_cast<int64_t>(K) * 2;
   const int64_t expert_rows = kDown ? p.hidden : 2 * static_cast<int64_t>(p.inter);
@@ -201,17 +232,16 @@ few_tokens_kernel(const Params p) {
   constexpr int kRowsAtOnce = 32 / S::kPieces;                     // weight rows of one copy instruction
   constexpr int kTokenCopies = S::kSlots * S::kTokenPieces / 32;   // copy instructions of the tokens
   const int w_row = lane / S::kPieces, w_col = lane % S::kPieces;
-  Place ahead = {0, 0, 0, 0, 1};
-  int ahead_tile = my_chunks ? blockIdx.x : tiles, ahead_chunk = 0, filled = 0;
-  int step = 0, step_by = 0;           // contraction step of the next chunk, and its increment
+  Place<kDown> ahead = {0, 0, 0, 0};
+  int ahead_tile = my_chunks ? tile0 : tiles, ahead_chunk = 0, filled = 0;
+  int step = 0;                        // contraction step of the next chunk
   const uint8_t* w_src = nullptr;      // of the next chunk
   const uint8_t* t_src[kTokenCopies];
   int live = 0;                        // tokens of the group
 
   auto locate = [&]() {  // the next chunk has another expert, group or tile than the last one
-    ahead.seek(r, kDown ? warp + ahead_chunk * kWarps : ahead_tile);
-    step = kDown ? ahead.unit : warp;
-    step_by = kDown ? kWarps / ahead.groups : kWarps;
+    ahead.seek(r, kDown ? chunk0 + ahead_chunk * next_chunk : ahead_tile, units);
+    step = kDown ? ahead.unit : chunk0;
     const int row0 = kDown ? ahead_tile * S::kRows : ahead.unit * (S::kRows / 2);
     w_src = reinterpret_cast<const uint8_t*>(p.w) + (r.expert[ahead.a] * expert_rows + row0 + w_row) * row_bytes +
             (static_cast<int64_t>(step) * S::kStep + w_col * 8) * 2;
@@ -269,14 +299,14 @@ few_tokens_kernel(const Params p) {
     if (ahead_tile >= tiles) return;
     if (++ahead_chunk >= my_chunks) {
       ahead_chunk = 0;
-      ahead_tile += gridDim.x;
+      ahead_tile += tile_step;
       if (kDown) ahead.a = 0;
       if (ahead_tile < tiles) locate();
-    } else if (kDown && warp + ahead_chunk * kWarps >= ahead.until) {
+    } else if (kDown && chunk0 + ahead_chunk * next_chunk >= ahead.until) {
       locate();
     } else {
-      step += step_by;
-      const uint32_t bytes = static_cast<uint32_t>(step_by) * (S::kStep * 2);
+      step += next_chunk;
+      const uint32_t bytes = static_cast<uint32_t>(next_chunk) * (S::kStep * 2);
       w_src += bytes;
 #pragma unroll
       for (int i = 0; i < kTokenCopies; ++i) t_src[i] += bytes * S::kParts;
@@ -293,12 +323,11 @@ few_tokens_kernel(const Params p) {
   if (ahead_tile < tiles) locate();
   if constexpr (kDown) {
     // Weights first, then, once kernel 1 is through, the activations that go with them.
-    const int tile0 = ahead_tile;
     for (int s = 0; s < S::kStages - 1; ++s) {
       if (ahead_tile < tiles) issue_weights(ring + filled * S::kStageBytes);
       advance();
     }
-    ahead_tile = tile0; ahead_chunk = 0; filled = 0; ahead.a = 0;
+    ahead_tile = my_chunks ? tile0 : tiles; ahead_chunk = 0; filled = 0; ahead.a = 0;
     if (ahead_tile < tiles) locate();
     pdl_wait();
     for (int s = 0; s < S::kStages - 1; ++s) {
@@ -317,7 +346,7 @@ few_tokens_kernel(const Params p) {
   // the same of the next 8.  Tokens: eight slots of 8 elements, four times in a row.
   const int m_row = lane & 15, m_col = lane >> 4;
   int stage = 0, parity = 0, here_live = 0;
-  Place here = {0, 0, 0, 0, 1};
+  Place<kDown> here = {0, 0, 0, 0};
   float acc[S::kSets][kRT][kCT][4];
   auto clear = [&]() {
 #pragma unroll
@@ -330,7 +359,7 @@ few_tokens_kernel(const Params p) {
           for (int j = 0; j < 4; ++j) acc[s][m][n][j] = 0.f;
   };
   auto look_up = [&](int at) {
-    here.seek(r, at);
+    here.seek(r, at, units);
     here_live = min(r.count[here.a] - here.group * kGroup, kGroup);
   };
   // Element (row, token) of a warp's tile in kernel 2; rows shifted against bank conflicts.
@@ -385,14 +414,14 @@ few_tokens_kernel(const Params p) {
     }
   };
 
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  for (int tile = tile0; tile < tiles; tile += tile_step) {
     clear();
-    if (kDown) { here = {0, 0, 0, 0, 1}; here_live = 0; } else look_up(tile);
+    if (kDown) { here = {0, 0, 0, 0}; here_live = 0; } else look_up(tile);
 
     for (int i = 0; i < my_chunks; ++i) {
-      if (kDown && warp + i * kWarps >= here.until) {
+      if (kDown && chunk0 + i * next_chunk >= here.until) {
         flush();
-        look_up(warp + i * kWarps);
+        look_up(chunk0 + i * next_chunk);
       }
       issue_next();
       cp_async_wait<S::kStages - 1>();
@@ -408,43 +437,49 @@ few_tokens_kernel(const Params p) {
     if constexpr (kDown) {
       flush();
       __syncthreads();
-      for (int i = threadIdx.x; i < S::kRows * S::kMaxT; i += kThreads) {
-        const int row = i % S::kRows, token = i / S::kRows;
-        float v = 0.f;
+      if (p.cluster == 1) {
+        for (int i = threadIdx.x; i < S::kRows * S::kMaxT; i += kThreads) {
+          const int row = i % S::kRows, token = i / S::kRows;
+          float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          v += sum_at(w, row, token);
-          sum_at(w, row, token) = 0.f;
-        }
-        if (token < p.tokens)
-          p.out[static_cast<int64_t>(token) * p.hidden + tile * S::kRows + row] = __float2bfloat16_rn(v);
-      }
-      __syncthreads();
-    } else {
-      // Two buffers in turn make one barrier per tile enough.
-      float4* sums = reinterpret_cast<float4*>(s_sum) + parity * kWarps * kRT * kCT * 32;
-      parity ^= 1;
-#pragma unroll
-      for (int m = 0; m < kRT; ++m)
-#pragma unroll
-        for (int n = 0; n < kCT; ++n) {
-          float4 v = make_float4(acc[0][m][n][0], acc[0][m][n][1], acc[0][m][n][2], acc[0][m][n][3]);
-          if (S::kSets == 2) {
-            v.x += acc[S::kSets - 1][m][n][0]; v.y += acc[S::kSets - 1][m][n][1];
-            v.z += acc[S::kSets - 1][m][n][2]; v.w += acc[S::kSets - 1][m][n][3];
+          for (int w = 0; w < kWarps; ++w) {
+            v += sum_at(w, row, token);
+            sum_at(w, row, token) = 0.f;
           }
-          sums[(warp * kRT * kCT + m * kCT + n) * 32 + lane] = v;
+          if (token < p.tokens)
+            p.out[static_cast<int64_t>(token) * p.hidden + tile * S::kRows + row] = __float2bfloat16_rn(v);
         }
-      __syncthreads();
-      if (warp < kRT * kCT) {
-        float4 v = sums[warp * 32 + lane];
+        __syncthreads();
+      } else {
+        // Every CTA of the cluster adds up its warps in place of the first, then a share of the tile over the
+        // CTAs, in their order.
+        for (int i = threadIdx.x; i < S::kRows * S::kMaxT; i += kThreads) {
+          const int row = i % S::kRows, token = i / S::kRows;
+          float v = 0.f;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
-          const float4 o = sums[(w * kRT * kCT + warp) * 32 + lane];
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+          for (int w = 0; w < kWarps; ++w) {
+            v += sum_at(w, row, token);
+            sum_at(w, row, token) = 0.f;
+          }
+          sum_at(0, row, token) = v;
         }
-        const int m = warp / kCT, n = warp % kCT;
-        // Gate element g and up element g of row tile m, for slots 2 t and 2 t + 1.
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const int outputs = S::kRows * p.tokens, rank = static_cast<int>(blockIdx.x % p.cluster);
+        for (int i = rank * kThreads + threadIdx.x; i < outputs; i += p.cluster * kThreads) {
+          const int row = i % S::kRows, token = i / S::kRows;
+          float v = 0.f;
+          for (int c = 0; c < p.cluster; ++c) v += *cluster.map_shared_rank(&sum_at(0, row, token), c);
+          p.out[static_cast<int64_t>(token) * p.hidden + tile * S::kRows + row] = __float2bfloat16_rn(v);
+        }
+        cluster.sync();
+        for (int i = threadIdx.x; i < S::kSumFloats; i += kThreads) s_sum[i] = 0.f;
+        __syncthreads();
+      }
+    } else {
+      // Gate element g and up element g of row tile m (v.x, v.y and v.z, v.w), for slots 2 t and 2 t + 1 of column
+      // tile n.
+      auto finish = [&](int m, int n, float4 v) {
         const float gate[2] = {v.x, v.y}, up[2] = {v.z, v.w};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -459,36 +494,107 @@ few_tokens_kernel(const Params p) {
             o[8 + g] = __float2bfloat16_rn(rest);
           }
         }
+      };
+      auto own = [&](int m, int n) {
+        float4 v = make_float4(acc[0][m][n][0], acc[0][m][n][1], acc[0][m][n][2], acc[0][m][n][3]);
+        if (S::kSets == 2) {
+          v.x += acc[S::kSets - 1][m][n][0]; v.y += acc[S::kSets - 1][m][n][1];
+          v.z += acc[S::kSets - 1][m][n][2]; v.w += acc[S::kSets - 1][m][n][3];
+        }
+        return v;
+      };
+      if constexpr (S::kAlone) {
+#pragma unroll
+        for (int m = 0; m < kRT; ++m)
+#pragma unroll
+          for (int n = 0; n < kCT; ++n) finish(m, n, own(m, n));
+      } else {
+        // Two buffers in turn make one barrier per tile enough.
+        float4* sums = reinterpret_cast<float4*>(s_sum) + parity * kWarps * kRT * kCT * 32;
+        parity ^= 1;
+#pragma unroll
+        for (int m = 0; m < kRT; ++m)
+#pragma unroll
+          for (int n = 0; n < kCT; ++n) sums[(warp * kRT * kCT + m * kCT + n) * 32 + lane] = own(m, n);
+        __syncthreads();
+        if (warp < kRT * kCT) {
+          float4 v = sums[warp * 32 + lane];
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) {
+            const float4 o = sums[(w * kRT * kCT + warp) * 32 + lane];
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+          }
+          finish(warp / kCT, warp % kCT, v);
+        }
       }
     }
   }
   cp_async_wait<0>();
 }
 
-template <int kCT, int kRT, bool kDown>
-int launch(const Params& p, int64_t tiles, cudaStream_t st) {
+template <typename S>
+int launch(Params p, const void* w, int64_t tiles, int cluster, cudaStream_t st) {
   const char* name = "moe_few_tokens";
-  const auto kernel = few_tokens_kernel<kCT, kRT, kDown>;
+  const auto kernel = few_tokens_kernel<S>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
   if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   const int64_t sms = sm_count();
-  launch_pdl(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), dim3(kThreads), kRingBytes, st, p);
+  p.cluster = cluster;
+  p.w = static_cast<const __nv_bfloat16*>(w);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((tiles < sms ? tiles : sms) * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kRingBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch(name);
 }
 
-// 32-row tiles where there are more than 8 tokens and the sizes allow it.
+template <int kCT, int kRT>
+int launch_up(const Params& p, const void* w13, int experts_hit, cudaStream_t st) {
+  const int64_t tiles = static_cast<int64_t>(experts_hit) * p.inter / (8 * kRT), sms = sm_count();
+  const int steps = (p.hidden + 128 / kRT - 1) / (128 / kRT);
+  // Where a tile has no more steps than the CTA has warps, adding them up takes longer than the tile: with tiles
+  // for every warp of the GPU, each warp takes its own (8 tokens, hidden 256, width 14336: 96 us together, 43
+  // alone; hidden 1024, width 3584: 37 and 32).  Longer tiles are better shared (hidden 4096, width 1792: 52
+  // together, 55 alone), because they come out even.
+  const bool alone = steps <= kWarps && tiles >= kWarps * sms;
+  return alone ? launch<Shape<kCT, kRT, false, true>>(p, w13, tiles, 1, st)
+               : launch<Shape<kCT, kRT, false, false>>(p, w13, tiles, 1, st);
+}
+
+template <int kCT, int kRT>
+int launch_down(const Params& p, const void* w2, int experts_hit, cudaStream_t st) {
+  const int64_t tiles = p.hidden / (16 * kRT);
+  // Where there are tiles for half of the SMs or fewer, clusters of two to eight CTAs share them, as long as every
+  // warp has eight steps (32 tokens, hidden 1024, width 3584: 57 us without clusters, 38 with them; 3 tokens,
+  // hidden and width 256: 8.4 and 13.6, a cluster takes longer to start and to add up).
+  const int64_t steps = static_cast<int64_t>(experts_hit) * (p.inter / (128 / kRT));
+  int cluster = 1;
+  while (cluster < kMaxCluster && tiles * cluster * 2 <= sm_count() && steps >= 8ll * kWarps * cluster * 2) cluster *= 2;
+  return launch<Shape<kCT, kRT, true, false>>(p, w2, tiles, cluster, st);
+}
+
+// 32-row tiles where there are more than 8 tokens, the sizes allow it and, in kernel 2, tiles for three quarters of
+// the SMs are left (16 tokens, hidden and width 2048: 49 us with 32-row tiles in kernel 2, 39 with 16-row tiles).
 template <int kCT>
-int launch(Params p, const void* w13, const void* w2, cudaStream_t st) {
+int launch(const Params& p, const void* w13, const void* w2, cudaStream_t st) {
   constexpr int kRT = kCT;
   const int experts_hit = 2 * p.tokens < kExperts ? 2 * p.tokens : kExperts;
-  const int64_t up_tiles = static_cast<int64_t>(experts_hit) * p.inter / 8;
-  p.w = static_cast<const __nv_bfloat16*>(w13);
-  if (int rc = p.inter % (8 * kRT) == 0 ? launch<kCT, kRT, false>(p, up_tiles / kRT, st)
-                                        : launch<kCT, 1, false>(p, up_tiles, st))
+  if (int rc = p.inter % (8 * kRT) == 0 ? launch_up<kCT, kRT>(p, w13, experts_hit, st)
+                                        : launch_up<kCT, 1>(p, w13, experts_hit, st))
     return rc;
-  p.w = static_cast<const __nv_bfloat16*>(w2);
-  return p.hidden % (16 * kRT) == 0 ? launch<kCT, kRT, true>(p, p.hidden / (16 * kRT), st)
-                                    : launch<kCT, 1, true>(p, p.hidden / 16, st);
+  const bool wide = p.hidden % (16 * kRT) == 0 && p.hidden / (16 * kRT) * 4 >= 3 * sm_count();
+  return wide ? launch_down<kCT, kRT>(p, w2, experts_hit, st) : launch_down<kCT, 1>(p, w2, experts_hit, st);
 }
 
 }  // namespace

@@ -93,6 +93,16 @@ def test_ties_and_masked_logits():
     assert (got[5].double() - d["w2"][3].double() @ act).norm() <= 2.0 ** -8 * (d["w2"][3].double() @ act).norm()
 
 
+@pytest.mark.parametrize("tokens,hidden,inter", [(17, 256, 128), (32, 4096, 256), (32, 512, 1000), (32, 2400, 520), (25, 1040, 72)])
+def test_all_tokens_on_two_experts(tokens, hidden, inter):
+    """More tokens of an expert than a ring stage holds: its weights are gone through twice."""
+    c = case(tokens, hidden, inter, seed=tokens)
+    c["logits"][:, 3] = 8.0
+    c["logits"][:, 6] = 9.0
+    c["logits"][tokens // 2, 1] = 20.0
+    check(c, run(c))
+
+
 def test_large_and_saturated_gates():
     c = case(6, 256, 128, seed=8)
     c["x"] *= 60
