@@ -1,6 +1,8 @@
 // Shared helpers of libb200moe: error reporting, launch checks and small device utilities.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -30,6 +32,18 @@ inline int check_launch(const char* what) {
 
 // Number of SMs of the current device (cached per device).
 int sm_count();
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device, once per device: `done` is a
+// static of the caller, one for each kernel.
+template <typename K>
+inline cudaError_t allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))
+    return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 

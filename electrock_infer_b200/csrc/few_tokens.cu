@@ -536,7 +536,8 @@ template <typename S>
 int launch(Params p, const void* w, int64_t tiles, int cluster, cudaStream_t st) {
   const char* name = "moe_few_tokens";
   const auto kernel = few_tokens_kernel<S>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared_memory(kernel, kRingBytes, done);
   if (e != cudaSuccess) return fail(B200MOE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   const int64_t sms = sm_count();
   p.cluster = cluster;
