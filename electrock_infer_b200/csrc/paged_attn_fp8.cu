@@ -32,7 +32,8 @@
 // through a workspace and a second kernel.
 // (The tensor cores of sm_100a take codes directly only through tcgen05; m16n8k32 of codes is carried out as
 // conversions and products of fp16, and measured a tenth slower than converting here.)
-// Bound by HBM: 256 bytes per token and KV head.
+// Bound by HBM: 256 bytes per token and KV head.  128 sequences of 4096-8192 tokens with 8 x 4 heads: 256 us, 6.3
+// TB/s; 4 of 30000-60000 with 16 query heads on one KV head: 19.9 us, bound by instructions; 1 of 700: 5.2 us.
 #include <cooperative_groups.h>
 
 #include "fp8_cache.cuh"
@@ -81,6 +82,7 @@ struct Params {
   int64_t q_stride, num_blocks, table_stride;
   int q_heads, kv_heads, group, block_size, max_blocks, num_splits;
   FastDiv by_block;
+  bool chunk_in_page;  // pages are whole chunks
   float scale_log2;
 };
 
@@ -136,27 +138,44 @@ paged_attn_fp8_kernel(const Params p) {
 
   // Issues the copies of the CTA's chunk `ci` into ring slot `stage`.  A page outside the cache is
   // replaced by page 0, tokens past the range are filled with zeros (0 * NaN would poison the output).
+  auto page_of = [&](int tok, int& off) {
+    const int index = p.by_block(tok);
+    const int page = table[index];
+    off = tok - index * p.block_size;
+    return page < 0 || page >= p.num_blocks ? 0 : page;
+  };
+  auto copy_tile = [&](const uint8_t* k, uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < kTile / 4; ++j, k += four_rows) {
+      const uint32_t dst = (j & 1 ? dst_odd : dst_even) + to + (j & ~1) * 4 * kDim;
+      cp_async_16(dst, k, 16);
+      cp_async_16(dst + kHalfBytes, k + v_minus_k, 16);
+    }
+  };
   auto issue = [&](int ci, int stage) {
-    if (ci < num_chunks) {
+    const int tok0 = t_begin + ci * kChunk;
+    const uint32_t scales_to = scales_addr + stage * 2 * kChunkTiles * 4;
+    if (ci < num_chunks && p.chunk_in_page && tok0 + kChunk <= t_end) {
+      // A whole chunk, in one page.
+      int off;
+      const int page = page_of(tok0, off);
+      const uint8_t* k = p.k_cache + (static_cast<int64_t>(page) * p.block_size + off) * row_bytes + row_at;
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile, k += 4 * four_rows)
+        copy_tile(k, stage * kStageBytes + tile * kTile * kDim);
+      if (lane < 2 * kChunkTiles)
+        cp_async_4(scales_to + lane * 4,
+                   (lane & 1 ? p.v_scale : p.k_scale) + static_cast<int64_t>(page) * p.kv_heads + kvh);
+    } else if (ci < num_chunks) {
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile) {
-        const int tok = t_begin + ci * kChunk + tile * kTile;
+        const int tok = tok0 + tile * kTile;
         int page = 0, off = 0;
-        if (tok < t_end) {
-          const int index = p.by_block(tok);
-          page = table[index];
-          off = tok - index * p.block_size;
-          if (page < 0 || page >= p.num_blocks) page = 0;
-        }
+        if (tok < t_end) page = page_of(tok, off);
         const uint8_t* k = p.k_cache + (static_cast<int64_t>(page) * p.block_size + off) * row_bytes + row_at;
         const uint32_t to = stage * kStageBytes + tile * kTile * kDim;
         if (tok + kTile <= t_end) {
-#pragma unroll
-          for (int j = 0; j < kTile / 4; ++j, k += four_rows) {
-            const uint32_t dst = (j & 1 ? dst_odd : dst_even) + to + (j & ~1) * 4 * kDim;
-            cp_async_16(dst, k, 16);
-            cp_async_16(dst + kHalfBytes, k + v_minus_k, 16);
-          }
+          copy_tile(k, to);
         } else {
 #pragma unroll
           for (int j = 0; j < kTile / 4; ++j) {
@@ -167,10 +186,9 @@ paged_attn_fp8_kernel(const Params p) {
             cp_async_16(dst + kHalfBytes, from + v_minus_k, bytes);
           }
         }
-        if (lane < 2) {
-          const float* s = (lane ? p.v_scale : p.k_scale) + static_cast<int64_t>(page) * p.kv_heads + kvh;
-          cp_async_4(scales_addr + (stage * 2 * kChunkTiles + tile * 2 + lane) * 4, s);
-        }
+        if (lane < 2)
+          cp_async_4(scales_to + (tile * 2 + lane) * 4,
+                     (lane ? p.v_scale : p.k_scale) + static_cast<int64_t>(page) * p.kv_heads + kvh);
       }
     }
     cp_async_commit();
@@ -185,7 +203,7 @@ paged_attn_fp8_kernel(const Params p) {
   // Query rows as B fragments: column n = head, and the contraction index of step 4 * i + w in lane t
   // is the dims (2 t + i) * 16 + 4 w .. + 3, the order in which the lane reads its tokens' codes.
   uint32_t qb[kNT][kDim / 16][2];
-  float qmul[kNT][2];  // score factor of heads 2 t and 2 t + 1 (the columns of a lane's accumulators)
+  float qmul[kNT][2];  // score factor of heads 2 t and 2 t + 1 (the columns of a lane's accumulators); its sign is in q
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     const bool live = n * 8 + g < p.group;
@@ -211,10 +229,10 @@ paged_attn_fp8_kernel(const Params p) {
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     // 2^up brings the row's largest value to [2^14, 2^15).
     const int up = amax >> 23 ? min(max(14 + 127 - static_cast<int>(amax >> 23), -126), 126) : 0;
-    const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    const float f = copysignf(__uint_as_float(static_cast<uint32_t>(127 + up) << 23), p.scale_log2);
     const float back = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-    qmul[n][0] = __shfl_sync(0xffffffffu, back, 8 * t) * p.scale_log2;
-    qmul[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * p.scale_log2;
+    qmul[n][0] = __shfl_sync(0xffffffffu, back, 8 * t) * fabsf(p.scale_log2);
+    qmul[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * fabsf(p.scale_log2);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -246,7 +264,10 @@ paged_attn_fp8_kernel(const Params p) {
     cp_async_wait<kStages - 1>();
     __syncwarp();
     const uint32_t ksm = ring + stage * kStageBytes, vsm = ksm + kHalfBytes;
-    const float* sc = scales + stage * 2 * kChunkTiles;
+    static_assert(kChunkTiles == 2, "the scales of a stage are K, V, K, V");
+    const float4 sc = *reinterpret_cast<const float4*>(scales + stage * 2 * kChunkTiles);
+    const float ks[kChunkTiles] = {usable_scale(sc.x), usable_scale(sc.z)};
+    const float vs_of[kChunkTiles] = {usable_scale(sc.y), usable_scale(sc.w)};
     const int tok0 = t_begin + (warp + i * kWarps) * kChunk;
 
     float s[kChunkTiles][kNT][4];
@@ -270,62 +291,67 @@ paged_attn_fp8_kernel(const Params p) {
           for (int n = 0; n < kNT; ++n) Mma<__half>::run(s[tile][n], a, qb[n][h * 4 + w][0], qb[n][h * 4 + w][1]);
         }
       }
-      // Into the exp2 domain.
-      const float ks = usable_scale(sc[tile * 2]);
-#pragma unroll
-      for (int n = 0; n < kNT; ++n) {
-        const float f0 = qmul[n][0] * ks, f1 = qmul[n][1] * ks;
-        s[tile][n][0] *= f0;
-        s[tile][n][1] *= f1;
-        s[tile][n][2] *= f0;
-        s[tile][n][3] *= f1;
-      }
     }
-    if (tok0 + kChunk > t_end) {  // tokens past the range do not count
+    const bool cut = tok0 + kChunk > t_end;  // tokens past the range do not count
+    auto past = [&](int tile, int j) { return tok0 + tile * kTile + g + (j >> 1) * 8 >= t_end; };
+    if (cut) {
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile)
 #pragma unroll
         for (int n = 0; n < kNT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (tok0 + tile * kTile + g + (j >> 1) * 8 >= t_end) s[tile][n][j] = -INFINITY;
+            if (past(tile, j)) s[tile][n][j] = -INFINITY;
     }
-    // A chunk holds at least one token of the range, so its maxima are finite.  The reference point of a
-    // head's exponentials follows the maximum only when that has risen by more than 2^kSlack: until then
-    // P may reach 2^kSlack, which costs no precision, and nothing has to be rescaled.
+    // Exponentials are taken relative to a reference point that follows the maximum only when that has risen
+    // by more than 2^kSlack: until then P may reach 2^kSlack, which costs no precision, nothing has to be
+    // rescaled, and the lanes need not agree on the chunk's maximum.  (A chunk holds at least one token of the
+    // range, so its maxima are finite.)
     uint32_t pb[kChunkTiles][kNT][2];  // P^T as B fragments
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float top[2];
+      float f[kChunkTiles][2], top[2];  // factors into the exp2 domain, not negative; this lane's maxima
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
 #pragma unroll
-        for (int tile = 1; tile < kChunkTiles; ++tile) top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]));
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+        for (int tile = 0; tile < kChunkTiles; ++tile) f[tile][c] = qmul[n][c] * ks[tile];
+        top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]) * f[0][c];
+#pragma unroll
+        for (int tile = 1; tile < kChunkTiles; ++tile)
+          top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]) * f[tile][c]);
       }
       if (__any_sync(0xffffffffu, top[0] > mx[n][0] + kSlack || top[1] > mx[n][1] + kSlack)) {
-        const float n0 = fmaxf(mx[n][0], top[0]), n1 = fmaxf(mx[n][1], top[1]);
-        const float a0 = exp2_fast(mx[n][0] - n0), a1 = exp2_fast(mx[n][1] - n1);  // 0 on the first chunk
-        mx[n][0] = n0;
-        mx[n][1] = n1;
-        sum[n][0] *= a0;
-        sum[n][1] *= a1;
 #pragma unroll
-        for (int m = 0; m < kDim / 16; ++m) {
-          o[n][m][0] *= a0; o[n][m][1] *= a1;
-          o[n][m][2] *= a0; o[n][m][3] *= a1;
+        for (int c = 0; c < 2; ++c) {
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+          top[c] = fmaxf(mx[n][c], top[c]);
+          const float a = exp2_fast(mx[n][c] - top[c]);  // 0 on the first chunk
+          mx[n][c] = top[c];
+          sum[n][c] *= a;
+#pragma unroll
+          for (int m = 0; m < kDim / 16; ++m) {
+            o[n][m][c] *= a;
+            o[n][m][c + 2] *= a;
+          }
         }
       }
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[tile][n][j] = exp2_fast(s[tile][n][j] - mx[n][j & 1]);
-          sum[n][j & 1] += s[tile][n][j];
-        }
+        for (int j = 0; j < 4; ++j) s[tile][n][j] = exp2_fast(fmaf(s[tile][n][j], f[tile][j & 1], -mx[n][j & 1]));
+      if (cut) {  // also where the factor is 0
+#pragma unroll
+        for (int tile = 0; tile < kChunkTiles; ++tile)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (past(tile, j)) s[tile][n][j] = 0.f;
+      }
+#pragma unroll
+      for (int tile = 0; tile < kChunkTiles; ++tile)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[n][j & 1] += s[tile][n][j];
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile) {
         pb[tile][n][0] = transpose_8x8(Mma<__half>::pack(s[tile][n][0], s[tile][n][1]));
@@ -334,7 +360,7 @@ paged_attn_fp8_kernel(const Params p) {
     }
 #pragma unroll
     for (int tile = 0; tile < kChunkTiles; ++tile) {
-      const float vs = usable_scale(sc[tile * 2 + 1]);
+      const float vs = vs_of[tile];
       if (vs != unit && tok0 + tile * kTile < t_end) {
         const float f = unit / vs;
         unit = vs;
@@ -581,15 +607,15 @@ extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_
   using namespace b200moe;
   if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || max_context < 1) return 1;
   // Estimated time of each number of splits, from measurements with 1 to 128 sequences of 100 to 60000
-  // tokens (1 x 8 heads x 700 tokens: 8.5 us unsplit, 5.5 us in 8 splits; 16 x 8 x 8192: 66 us unsplit, 43 us
-  // in 3; 128 x 8 x 8192: 283 us unsplit, 256 us in 3; 16 x 8 x 1024: 10.9 us unsplit, 11.7 us in 3).  In ns:
-  // a CTA takes 7.4 a token when it has an SM to itself, 11.6 and 13.8 with one and two others beside it
-  // (10.5 and 14.7 with two head tiles); beyond one wave the GPU is filled evenly, but for a last wave of half
-  // a CTA's time and 1.2 us per CTA and wave; merging takes 2.4 us in a cluster, else 3.2 us and 80 ns a split.
+  // tokens (1 x 8 heads x 700 tokens: 7.7 us unsplit, 5.4 us in 8 splits; 16 x 8 x 8192: 54 us unsplit, 43 us
+  // in 3; 128 x 8 x 8192: 275 us unsplit, 257 us in 4; 16 x 8 x 1024: 9.8 us unsplit, 10.8 us in 3).  In ns:
+  // a CTA takes 6.0 a token when it has an SM to itself, 10.2 and 13.6 with one and two others beside it
+  // (8.7 and 13 with two head tiles); beyond one wave the GPU is filled evenly, but for a last wave of half
+  // a CTA's time and 1.2 us per CTA and wave; merging takes 1.5 us in a cluster, else 1.6 us and 40 ns a split.
   const bool wide = q_heads / kv_heads > 8;
   const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, sms = sm_count();
   const int64_t slots = sms * (wide ? Ring<2>::kCtas : Ring<1>::kCtas);
-  const double by_share[3] = {wide ? 10.5 : 7.4, wide ? 14.7 : 11.6, 13.8};
+  const double by_share[3] = {wide ? 8.7 : 6.0, wide ? 13.0 : 10.2, 13.6};
   int best = 1;
   double best_cost = 0;
   for (int s = 1; s <= kMaxSplits; ++s) {
@@ -600,7 +626,7 @@ extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_
     double cost = tokens * by_share[per_sm - 1];
     if (ctas > slots) cost *= static_cast<double>(ctas) / slots + 0.5;
     if (ctas > slots) cost += 1200.0 * ctas / slots;
-    if (s > 1) cost += merges_in_cluster(pairs, s, sms) ? 2400.0 : 3200.0 + 80.0 * s;
+    if (s > 1) cost += merges_in_cluster(pairs, s, sms) ? 1500.0 : 1600.0 + 40.0 * s;
     if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
   }
   return best;
@@ -661,6 +687,7 @@ extern "C" int b200moe_paged_attn_varlen_fp8(const void* q, const void* k_cache,
   p.max_blocks = max_blocks_per_seq; p.num_splits = num_splits; p.num_blocks = num_blocks;
   p.scale_log2 = softmax_scale * kLog2e;
   p.by_block = FastDiv::by(static_cast<uint32_t>(block_size));
+  p.chunk_in_page = block_size % kChunk == 0;
   const size_t need = b200moe_paged_attn_fp8_workspace_bytes(batch, q_heads, kv_heads, num_splits);
   if (need > 0) {
     if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))

@@ -1,5 +1,5 @@
 """Bandwidth sweep of the HBM-bound ops (router, alignment, combine, stand-alone SwiGLU, gate
-router, RMSNorm, paged KV-cache store and decode attention).
+router, RMSNorm, paged KV-cache store and decode attention in 16 and 8 bits, few-token experts).
 
     python -m electrock_infer_b200.opbench [--tokens 1048576 2097152 4194304] [--iters 20]
 
@@ -131,6 +131,12 @@ def main() -> None:
         slots = torch.randperm(nblk * bs, generator=g, device=dev)[:tokens].to(torch.int32)
         ms = time_op(lambda: _C.paged_store_kvcache(key, val, kc, vc, slots), args.iters, flush)
         report("paged_store_kvcache", tokens, tokens * kv_heads * hd * 2 * 4 + tokens * 4, ms)
+        k8, v8 = kc.to(torch.float8_e4m3fn), vc.to(torch.float8_e4m3fn)
+        ks = torch.zeros(nblk, kv_heads, device=dev)
+        vs = torch.zeros_like(ks)
+        slots = torch.arange(tokens, dtype=torch.int32, device=dev)
+        ms = time_op(lambda: _C.paged_store_kvcache_fp8(key, val, k8, v8, ks, vs, slots), args.iters, flush)
+        report("paged_store_kvcache_fp8", tokens, tokens * kv_heads * hd * 2 * 3 + tokens * 4, ms)
     for batch, ctx in (tuple(int(v) for v in c.split(":")) for c in args.kv_cases):
         per_seq = (ctx + bs - 1) // bs
         nblk = batch * per_seq
@@ -145,6 +151,26 @@ def main() -> None:
                      args.iters, flush)
         nbytes = total * kv_heads * hd * 2 * 2 + batch * q_heads * hd * 2 * 2
         report("paged_attn_varlen", total, nbytes, ms, batch=batch, max_context=ctx)
+        k8, v8 = kc.to(torch.float8_e4m3fn), vc.to(torch.float8_e4m3fn)
+        del kc, vc
+        ones = torch.ones(nblk, kv_heads, device=dev)
+        ms = time_op(lambda: _C.paged_attn_varlen_fp8(q, k8, v8, ones, ones, ctx, lens, table, hd ** -0.5),
+                     args.iters, flush)
+        nbytes = total * kv_heads * hd * 2 + batch * q_heads * hd * 2 * 2
+        report("paged_attn_varlen_fp8", total, nbytes, ms, batch=batch, max_context=ctx)
+    # The expert layer for a few tokens, every expert hit or (one token) two of them.
+    for tokens, inter in ((1, 14336), (8, 14336), (32, 14336)):
+        w13 = torch.randn(8, 2 * inter, H, generator=g, device=dev, dtype=torch.bfloat16) * 0.01
+        w2 = torch.randn(8, H, inter, generator=g, device=dev, dtype=torch.bfloat16) * 0.01
+        x = torch.randn(tokens, H, generator=g, device=dev).to(torch.bfloat16)
+        logits = torch.zeros(tokens, 8, device=dev)
+        rows = torch.arange(tokens, device=dev)
+        logits[rows, (2 * rows) % 8] = 2.0
+        logits[rows, (2 * rows + 1) % 8] = 1.0
+        out = torch.empty_like(x)
+        ms = time_op(lambda: _C.moe_few_tokens(out, x, logits, w13, w2), args.iters, flush)
+        report("moe_few_tokens", tokens, min(2 * tokens, 8) * 6 * H * inter, ms, inter=inter)
+        del w13, w2
 
 
 if __name__ == "__main__":

@@ -255,6 +255,13 @@ def test_attention_with_small_and_large_queries(size):
     check_attn(c, attend(c))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_attention_with_other_softmax_scales(scale):
+    c = {**attn_case([77, 500, 5], 8, 2, 32, torch.float16, seed=3), "scale": scale}
+    for splits in (1, 3):
+        check_attn(c, attend(c, splits))
+
+
 def test_attention_where_scales_differ_by_page():
     """Pages whose scales lie up to 2^40 apart, the loud ones with vanishing weight."""
     c = attn_case([320, 47], 8, 2, 16, torch.bfloat16, seed=5)
