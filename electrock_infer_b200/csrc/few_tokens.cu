@@ -488,7 +488,7 @@ few_tokens_kernel(const Params p) {
           if (slot < here_live) {
             const float value = r.weight[here.a][place] * (gate[c] / (1.f + expf(-gate[c])) * up[c]);
             const __nv_bfloat16 high = __float2bfloat16_rn(value);
-            const float rest = value - __bfloat162float(high);
+            const float rest = __hisinf(high) ? 0.f : value - __bfloat162float(high);  // not inf - inf
             __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(
                 p.act + (static_cast<int64_t>(r.pair[here.a][place]) * (p.inter / 8) + here.unit * kRT + m) * 2);
             o[g] = high;

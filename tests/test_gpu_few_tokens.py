@@ -111,6 +111,21 @@ def test_large_and_saturated_gates():
     assert torch.isfinite(got.float()).all() and (got.double() - want).norm() <= 2.0 ** -8 * want.norm()
 
 
+def test_activations_beyond_the_range_become_infinities():
+    """An activation that overflows is an infinity, as in fp32, and does not turn into NaN on its way; other tokens
+    are not touched."""
+    c = case(3, 32, 16, seed=2)
+    c["w13"].zero_()
+    c["w13"][:, 0, 0] = c["w13"][:, 16, 0] = 1.0        # gate and up of element 0 are x[0]
+    c["w2"].zero_()
+    c["w2"][:, :, 0] = 1.0
+    c["w2"][:, 1, 0] = -1.0
+    c["x"][0, 0], c["x"][1, 0], c["x"][2, 0] = 1e25, 2.0, 1.85e19
+    got = run(c).float()
+    assert got[0, 0] == torch.inf and got[0, 1] == -torch.inf and not torch.isnan(got).any()
+    assert torch.isfinite(got[1]).all() and abs(got[1, 0].item() - 2 * 2 / (1 + 2.718281828 ** -2)) < 2 ** -8 * 4
+
+
 def test_in_place_and_no_tokens():
     c = case(9, 512, 256, seed=3)
     want = run(c)

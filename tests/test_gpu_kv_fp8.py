@@ -361,6 +361,30 @@ def test_attention_is_the_same_every_time_and_on_other_streams():
     assert all(torch.equal(o, first) for o in outs)
 
 
+def test_captured_attention_replayed_at_the_same_time():
+    """Two graphs with splits that go through a workspace, replayed on two streams at once: none shares scratch."""
+    c = attn_case([700, 90, 2000], 32, 8, 64, torch.bfloat16, seed=12)
+    d = {k: (t.to(DEV) if torch.is_tensor(t) else t) for k, t in c.items()}
+    qs = [d["q"], (d["q"].float() * -0.5).to(torch.bfloat16)]
+    call = lambda q: _C.paged_attn_varlen_fp8(q, d["k_cache"], d["v_cache"], d["k_scale"], d["v_scale"], 2000, d["lens"],  # noqa: E731
+                                              d["table"], d["scale"], num_splits=7)
+    want = [call(q) for q in qs]
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(q))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
 def test_attention_refusals():
     c = attn_case([10, 20], 32, 8, 32, torch.bfloat16, seed=1)
     d = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in c.items()}
