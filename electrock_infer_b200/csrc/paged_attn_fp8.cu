@@ -306,21 +306,25 @@ paged_attn_fp8_kernel(const Params p) {
     // Exponentials are taken relative to a reference point that follows the maximum only when that has risen
     // by more than 2^kSlack: until then P may reach 2^kSlack, which costs no precision, nothing has to be
     // rescaled, and the lanes need not agree on the chunk's maximum.  (A chunk holds at least one token of the
-    // range, so its maxima are finite.)
+    // range, so its maxima are finite.)  A score is rounded to fp32 before it is compared, made the reference point
+    // or measured against that: a product kept exact in one of these places would, from 2^28 on, be off the others
+    // by more than P has room for.
     uint32_t pb[kChunkTiles][kNT][2];  // P^T as B fragments
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float f[kChunkTiles][2], top[2];  // factors into the exp2 domain, not negative; this lane's maxima
+      float top[2];  // this lane's maxima
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        top[c] = -INFINITY;
 #pragma unroll
-        for (int tile = 0; tile < kChunkTiles; ++tile) f[tile][c] = qmul[n][c] * ks[tile];
-        top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]) * f[0][c];
-#pragma unroll
-        for (int tile = 1; tile < kChunkTiles; ++tile)
-          top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]) * f[tile][c]);
+        for (int tile = 0; tile < kChunkTiles; ++tile) {
+          const float f = qmul[n][c] * ks[tile];  // into the exp2 domain; not negative
+          s[tile][n][c] = __fmul_rn(s[tile][n][c], f);
+          s[tile][n][c + 2] = __fmul_rn(s[tile][n][c + 2], f);
+          top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]));
+        }
       }
-      if (__any_sync(0xffffffffu, top[0] > mx[n][0] + kSlack || top[1] > mx[n][1] + kSlack)) {
+      if (__any_sync(0xffffffffu, top[0] - mx[n][0] > kSlack || top[1] - mx[n][1] > kSlack)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
@@ -340,7 +344,7 @@ paged_attn_fp8_kernel(const Params p) {
 #pragma unroll
       for (int tile = 0; tile < kChunkTiles; ++tile)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[tile][n][j] = exp2_fast(fmaf(s[tile][n][j], f[tile][j & 1], -mx[n][j & 1]));
+        for (int j = 0; j < 4; ++j) s[tile][n][j] = exp2_fast(s[tile][n][j] - mx[n][j & 1]);
       if (cut) {  // also where the factor is 0
 #pragma unroll
         for (int tile = 0; tile < kChunkTiles; ++tile)
