@@ -20,9 +20,11 @@
 // contraction index of S and the output rows of O may be permuted at will, so a lane takes 16
 // consecutive codes of its token and the query is laid out to match; V's pairs of neighbouring tokens
 // are interleaved by byte permutes before they are widened.  fp16 holds every e4m3 value exactly, so
-// widening rounds nothing; q rows are scaled by a power of two into fp16's range (exact for
-// fp16 and bf16 values within 2^-38 of the row's largest), P is rounded to fp16 (2^-12 relative, below
-// the rounding of the output), all sums, maxima and the outputs are fp32.
+// widening rounds nothing; q rows are scaled by a power of two into fp16's range (exact for values within 2^-28,
+// fp16, or 2^-31, bf16, of the row's largest; smaller ones are kept to 2^-39 of it), P is rounded to fp16, all sums,
+// maxima and the outputs are fp32.  P's rounding, 2^-11 of a weight, is as large as that of an fp16 output and an eighth
+// of a bf16 one's, and the errors of many tokens average out; P in bf16 would err eight times as much, and a second
+// fp16 number for what is left would take half as many products again.
 //
 // Four warps stream their own 32-token chunks through rings of asynchronous 16-byte copies
 // (rows of 128 bytes, XOR-swizzled).  A page's K scale multiplies the scores; its V scale is the unit that
@@ -65,7 +67,12 @@ constexpr int kMaxCluster = 8;             // splits that merge through distribu
 constexpr int kMaxGroup = 16;
 constexpr int kMaxSplits = 64;
 constexpr int kMaxContext = 0x7fffffff - 4 * kTile;  // so that rounding up to chunks stays in range
-constexpr float kSlack = 8.f;              // in powers of two
+// Exponentials are taken relative to a reference point kLift powers of two below the running maximum, and that
+// point follows the maximum only when it has risen by more than kSlack: P reaches 2^(kLift + kSlack), half of
+// fp16's range.  Without the lift, weights under 2^-14 of the largest would be subnormal and those under 2^-25 lost,
+// which a long tail of them shows; with it these are 2^-21 and 2^-32.
+constexpr float kSlack = 8.f;
+constexpr float kLift = 7.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -78,7 +85,7 @@ struct Params {
   const int32_t* block_table;
   const int32_t* context_lens;
   float* ws_o;   // [batch, q_heads, splits, 128] un-normalised partial outputs
-  float* ws_ml;  // [batch, q_heads, splits, 2] running max (log2 domain) and sum
+  float* ws_ml;  // [batch, q_heads, splits, 2] reference point (log2 domain) and sum
   int64_t q_stride, num_blocks, table_stride;
   int q_heads, kv_heads, group, block_size, max_blocks, num_splits;
   FastDiv by_block;
@@ -250,7 +257,7 @@ paged_attn_fp8_kernel(const Params p) {
     for (int m = 0; m < kDim / 16; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[n][m][j] = 0.f;
-  float mx[kNT][2], sum[kNT][2];  // running maximum; this lane's part of the sum
+  float mx[kNT][2], sum[kNT][2];  // reference point of the exponentials; this lane's part of the sum
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     mx[n][0] = mx[n][1] = -INFINITY;
@@ -303,12 +310,10 @@ paged_attn_fp8_kernel(const Params p) {
           for (int j = 0; j < 4; ++j)
             if (past(tile, j)) s[tile][n][j] = -INFINITY;
     }
-    // Exponentials are taken relative to a reference point that follows the maximum only when that has risen
-    // by more than 2^kSlack: until then P may reach 2^kSlack, which costs no precision, nothing has to be
-    // rescaled, and the lanes need not agree on the chunk's maximum.  (A chunk holds at least one token of the
-    // range, so its maxima are finite.)  A score is rounded to fp32 before it is compared, made the reference point
-    // or measured against that: a product kept exact in one of these places would, from 2^28 on, be off the others
-    // by more than P has room for.
+    // As long as the reference point stays where it is nothing has to be rescaled, and the lanes need not agree on the
+    // chunk's maximum.  (A chunk holds at least one token of the range, so its maxima are finite.)  A score is rounded
+    // to fp32 before it is compared, moves the reference point or is measured against that: a product kept exact in
+    // one of these places would, from 2^24 on, be off the others by more than P has room for.
     uint32_t pb[kChunkTiles][kNT][2];  // P^T as B fragments
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
@@ -324,13 +329,13 @@ paged_attn_fp8_kernel(const Params p) {
           top[c] = fmaxf(top[c], fmaxf(s[tile][n][c], s[tile][n][c + 2]));
         }
       }
-      if (__any_sync(0xffffffffu, top[0] - mx[n][0] > kSlack || top[1] - mx[n][1] > kSlack)) {
+      if (__any_sync(0xffffffffu, top[0] - mx[n][0] > kLift + kSlack || top[1] - mx[n][1] > kLift + kSlack)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
           top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
           top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-          top[c] = fmaxf(mx[n][c], top[c]);
+          top[c] = fmaxf(mx[n][c], top[c] - kLift);
           const float a = exp2_fast(mx[n][c] - top[c]);  // 0 on the first chunk
           mx[n][c] = top[c];
           sum[n][c] *= a;
@@ -407,9 +412,9 @@ paged_attn_fp8_kernel(const Params p) {
   // 16 and rows by 20 against bank conflicts.
   constexpr int kHeads = kNT * 8, kPitch = kDim + 20;
   float* sm_o = reinterpret_cast<float*>(smem);              // [warps][kHeads][kPitch]
-  float* sm_ml = sm_o + kWarps * kHeads * kPitch;            // [warps][kHeads][2]: maximum, sum
+  float* sm_ml = sm_o + kWarps * kHeads * kPitch;            // [warps][kHeads][2]: reference point, sum
   float* sm_f = sm_ml + kWarps * kHeads * 2;                 // [kHeads][warps]: the warps' weights
-  float* sm_total = sm_f + kHeads * kWarps;                  // [kHeads][2]: the CTA's maximum and sum
+  float* sm_total = sm_f + kHeads * kWarps;                  // [kHeads][2]: the CTA's reference point and sum
   float* sm_acc = sm_total + kHeads * 2;                     // [kHeads][128]: the CTA's output
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
