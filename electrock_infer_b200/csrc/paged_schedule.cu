@@ -267,7 +267,7 @@ paged_schedule_kernel(const Params p) {
   const int first = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
   const int used_rows = min(total[0], p.num_rows);
   const int per_group = p.num_rows > stride ? kRowsPerThread : 1;
-  const int64_t groups = (p.num_rows + per_group - 1) / per_group;
+  const int64_t groups = per_group == 1 ? p.num_rows : (p.num_rows - 1) / kRowsPerThread + 1;
   const int64_t pops = groups + s_taken, pushes = pops + (avail - top), all = pushes + R;
   for (int64_t w = first; w < all; w += stride) {
     if (w < groups) {
