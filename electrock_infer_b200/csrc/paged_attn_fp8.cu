@@ -643,7 +643,7 @@ extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_
 
 extern "C" size_t b200moe_paged_attn_fp8_workspace_bytes(int batch, int q_heads, int kv_heads, int num_splits) {
   using namespace b200moe;
-  if (batch < 1 || q_heads < 1 || kv_heads < 1 || num_splits <= 1 ||
+  if (batch < 1 || q_heads < 1 || kv_heads < 1 || num_splits <= 1 || num_splits > kMaxSplits ||
       merges_in_cluster(static_cast<int64_t>(batch) * kv_heads, num_splits, sm_count()))
     return 0;
   return static_cast<size_t>(batch) * q_heads * num_splits * (kDim + 2) * sizeof(float);

@@ -446,7 +446,8 @@ int b200moe_paged_schedule(const int32_t* context_lens, const int32_t* new_lens,
  * are fp32, the probabilities are rounded to fp16 for the product with V.  A NaN in a context gives NaN;
  * codes past a context may be anything.  num_splits is 1 to 64 (b200moe_paged_attn_fp8_num_splits suggests
  * a value); above 1 it may need a workspace of b200moe_paged_attn_fp8_workspace_bytes bytes, which is 0
- * where the splits merge inside the kernel.  Both functions ask for the current device's SM count.
+ * where the splits merge inside the kernel and for numbers of splits that the call refuses.  Both functions
+ * ask for the current device's SM count.
  */
 int b200moe_paged_store_kvcache_fp8(const void* key, const void* value, void* k_cache, void* v_cache,
                                     float* k_scale, float* v_scale, const int32_t* slot_mapping,

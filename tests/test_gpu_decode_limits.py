@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from electrock_infer_b200 import _C
+from test_gpu_kv_fp8 import attn_case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -28,3 +29,16 @@ def test_schedule_with_as_many_rows_as_it_takes(rows):
     assert slots[:63].tolist() == want
     for part in slots[63:].split(1 << 28):
         assert int(part.max()) == -1 == int(part.min())
+
+
+@pytest.mark.parametrize("splits", [65, 10 ** 6, 2 ** 31 - 1])
+def test_attention_refuses_too_many_splits_before_it_allocates_their_scratch(splits):
+    c = attn_case([10, 20], 32, 8, 32, torch.bfloat16, seed=1)
+    d = {k: (v.to(DEV) if torch.is_tensor(v) else v) for k, v in c.items()}
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(RuntimeError, match="num_splits"):
+        _C.paged_attn_varlen_fp8(d["q"], d["k_cache"], d["v_cache"], d["k_scale"], d["v_scale"], 0, d["lens"], d["table"], 0.1,
+                                 num_splits=splits)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * 32 * 128 * 2      # the output
