@@ -47,6 +47,10 @@ def _native():
         except ImportError as e:
             raise RuntimeError(f"the compiled binding is missing or does not fit this torch ({e}): build it with "
                                "`python -m electrock_infer_b200.build`") from None
+        from .build import binding_target
+        if module.built_for != binding_target():
+            raise RuntimeError(f"the compiled binding was built for {module.built_for}, this is {binding_target()}: build "
+                               "it with `python -m electrock_infer_b200.build`")
         _binding = module
     return _binding
 

@@ -18,6 +18,7 @@ LIB_PATH = PKG_DIR / "libb200moe.so"
 INCLUDE_DIR = PKG_DIR.parent / "include"
 BINDING_PATH = PKG_DIR / "_binding.so"
 BINDING_SOURCE = CSRC / "torch_binding.cpp"
+BINDING_STAMP = PKG_DIR / "_binding.built_for"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -47,8 +48,17 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > built for p in deps)
 
 
+def binding_target() -> str:
+    """The torch, C++ ABI and interpreter that a binding is compiled against; one that was compiled against
+    others may load and misread tensors."""
+    import sysconfig
+
+    import torch
+    return f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, {sysconfig.get_config_var('SOABI')}"
+
+
 def binding_is_stale() -> bool:
-    if not BINDING_PATH.exists():
+    if not BINDING_PATH.exists() or not BINDING_STAMP.exists() or BINDING_STAMP.read_text() != binding_target():
         return True
     built = BINDING_PATH.stat().st_mtime
     return any(p.stat().st_mtime > built for p in [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h")])
@@ -67,12 +77,14 @@ def build_binding(force: bool = False) -> Path:
                 cuda / "include"]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DB200MOE_BUILT_FOR="{binding_target()}"',
            "-o", str(BINDING_PATH), str(BINDING_SOURCE), *(f"-I{d}" for d in includes),
            f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", f"-L{home / 'lib'}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    BINDING_STAMP.write_text(binding_target())
     return BINDING_PATH
 
 

@@ -309,4 +309,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-extern "C" PyObject* PyInit__binding() { return PyModule_Create(&module); }
+extern "C" PyObject* PyInit__binding() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", B200MOE_BUILT_FOR) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
