@@ -31,7 +31,8 @@ class FusedMoE(nn.Module):
 
     Extension: batches of up to ``few_token_limit`` tokens (0 to 32; default 0: none) take the two-kernel
     path ``fused_experts(few_tokens=True)``, whose results differ from the general path's in the last
-    bits.  Needs 8 experts and top-2; a sum over ranks is then NCCL's.
+    bits.  Needs 8 experts and top-2; a sum over ranks is then NCCL's, so that where there is one the limit
+    does not go with ``tp_exchange="peer"``.
     """
 
     PEER_REDUCE_MIN_BYTES = 4 << 20
@@ -67,6 +68,9 @@ class FusedMoE(nn.Module):
         if self.intermediate_size % self.tp_size != 0:
             raise ValueError(f"intermediate_size ({self.intermediate_size}) must be divisible by "
                              f"tp_size ({self.tp_size})")
+        if few_token_limit and tp_exchange == "peer" and reduce_results and self.tp_size > 1:
+            raise ValueError("few_token_limit does not go with tp_exchange='peer': the sum over ranks of such batches "
+                             "is NCCL's")
         self.intermediate_size_per_partition = self.intermediate_size // self.tp_size
 
         self.w13_weight = nn.Parameter(
