@@ -440,7 +440,9 @@ def paged_store_kvcache_fp8(K: torch.Tensor, V: torch.Tensor, K_cache: torch.Ten
     stored as NaN, infinities and values out of range as the largest code of their sign.
 
     Slots must be distinct, and the tokens of one page must follow one another in the call with nothing
-    but skipped entries between them, as in every slot map that is built request by request.
+    but skipped entries between them, as in every slot map that is built request by request.  Unlike
+    ``paged_store_kvcache``, which takes slots in any order, this op leaves undefined what a page holds where that is
+    not so; it is not found out.  At most 65535 * 256 tokens a call.
     """
     (_binding or _native()).paged_store_kvcache_fp8(K, V, K_cache, V_cache, K_scale, V_scale, slot_mapping)
 
@@ -454,8 +456,9 @@ def paged_attn_varlen_fp8(Q: torch.Tensor, K_cache: torch.Tensor, V_cache: torch
 
     ``Q`` bf16 or fp16 ``[batch, q_heads, 128]`` (the batch stride may exceed a row); caches, scales as
     in the store; ``context_lens`` int32 ``[batch]``; ``block_table`` int32 ``[batch, max_blocks]`` (row
-    stride free).  Up to 16 query heads per KV head, block sizes that are multiples of 16.  An empty
-    context gives a zero row.  ``max_seqlen_k`` (0 = unknown) only helps to choose ``num_splits`` (0 =
+    stride free, at least a row).  One query row for each sequence: there is no form for several, which prompts
+    need in all but a model's last layer.  Up to 16 query heads per KV head, block sizes that are multiples of 16.
+    An empty context gives a zero row.  ``max_seqlen_k`` (0 = unknown) only helps to choose ``num_splits`` (0 =
     choose), the number of ranges that a context is cut into.  The scratch of the merge is allocated per
     call from torch's allocator, so that calls on different streams and captured graphs never share it.
     """

@@ -19,9 +19,12 @@
 // between the two: short runs (decode: one token) by one warp, longer ones by the whole CTA.  A run that
 // does not fit is read a second time (from L2).  Every CTA finds the runs of its segment of tokens for
 // itself, 3 us that a list written by a kernel of its own did not make up for.  Prompts: bound by the
-// phases of a CTA that follow one another (16 prompts of 512-1024 tokens with 8 heads in 28.3 us, of which
-// finding the runs 8, reading 10, converting and writing 7; 75.7 MB would take 11.6); decode steps by
-// latency (slot -> rows and old scale -> codes; 64 tokens in 3.3 us).
+// phases of a CTA that follow one another (16 prompts of 512-1024 tokens with 8 heads in 28.0 us, of which
+// finding the runs 8, reading 10, converting and writing 7; 75.7 MB would take 11.6).  Decode steps: bound by
+// latency (slot -> rows and old scale -> codes; 64 tokens in 3.3 us) as long as no scale grows.  Where one does, a
+// warp goes through the page four rows at a time, each load behind the last store: 1.5 us more with pages of 16
+// tokens, 7 with 64, 33 with 256, whether one page grows or four do (43 when all 1024 do).  Skipped entries behind the
+// last token cost 2 to 3 us up to 448 of them, 5 for 960, 19 for 4032: its run is followed to its end.
 #include "fp8_cache.cuh"
 
 namespace b200moe {

@@ -34,8 +34,8 @@
 // through a workspace and a second kernel.
 // (The tensor cores of sm_100a take codes directly only through tcgen05; m16n8k32 of codes is carried out as
 // conversions and products of fp16, and measured a tenth slower than converting here.)
-// Bound by HBM: 256 bytes per token and KV head.  128 sequences of 4096-8192 tokens with 8 x 4 heads: 256 us, 6.3
-// TB/s; 4 of 30000-60000 with 16 query heads on one KV head: 19.9 us, bound by instructions; 1 of 700: 5.2 us.
+// Bound by HBM: 256 bytes per token and KV head.  128 sequences of 4096-8192 tokens with 8 x 4 heads: 251 us, 6.4
+// TB/s; 4 of 30000-60000 with 16 query heads on one KV head: 20.1 us, bound by instructions; 1 of 700: 5.2 us.
 #include <cooperative_groups.h>
 
 #include "fp8_cache.cuh"
@@ -616,7 +616,7 @@ extern "C" int b200moe_paged_attn_fp8_num_splits(int batch, int q_heads, int kv_
   using namespace b200moe;
   if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || max_context < 1) return 1;
   // Estimated time of each number of splits, from measurements with 1 to 128 sequences of 100 to 60000
-  // tokens (1 x 8 heads x 700 tokens: 7.7 us unsplit, 5.4 us in 8 splits; 16 x 8 x 8192: 54 us unsplit, 43 us
+  // tokens (1 x 8 heads x 700 tokens: 7.7 us unsplit, 5.2 us in 8 splits; 16 x 8 x 8192: 54 us unsplit, 43 us
   // in 3; 128 x 8 x 8192: 275 us unsplit, 257 us in 4; 16 x 8 x 1024: 9.8 us unsplit, 10.8 us in 3).  In ns:
   // a CTA takes 6.0 a token when it has an SM to itself, 10.2 and 13.6 with one and two others beside it
   // (8.7 and 13 with two head tiles); beyond one wave the GPU is filled evenly, but for a last wave of half

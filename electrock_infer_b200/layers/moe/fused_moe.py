@@ -241,9 +241,9 @@ def fused_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
     ``parallel.TensorParallelReduce`` whose ``usable(num_tokens)`` holds on every rank) the result
     is also summed over the tensor-parallel ranks: the second GEMM stores its rows into the owning
     ranks' buffers over NVLink and the combine kernel finishes the all-reduce.  With ``few_tokens``
-    a batch of at most ``_C.few_tokens_max()`` tokens runs as two kernels that read each chosen
-    expert's weights once (``_C.moe_few_tokens``); it needs ``gating_output``, 8 experts and top-2, and
-    rounds only the result, so its results differ from the general path's in the last bits.
+    a batch of at most ``_C.few_tokens_max()`` tokens (a larger one is refused) runs as two kernels that
+    read each chosen expert's weights once (``_C.moe_few_tokens``); it needs ``gating_output``, 8 experts
+    and top-2, and rounds only the result, so its results differ from the general path's in the last bits.
     """
     if activation != "silu":
         raise NotImplementedError(f"Activation {activation} not supported.")

@@ -32,7 +32,8 @@ class FusedMoE(nn.Module):
     Extension: batches of up to ``few_token_limit`` tokens (0 to 32; default 0: none) take the two-kernel
     path ``fused_experts(few_tokens=True)``, whose results differ from the general path's in the last
     bits.  Needs 8 experts and top-2; a sum over ranks is then NCCL's, so that where there is one the limit
-    does not go with ``tp_exchange="peer"``.
+    does not go with ``tp_exchange="peer"``.  At hidden 4096 it is the faster path up to 32 tokens, by 10 %
+    (32 tokens, width 14336) to a third of the time (one token, width 1792).
     """
 
     PEER_REDUCE_MIN_BYTES = 4 << 20
@@ -162,7 +163,7 @@ class MixtralMoE(nn.Module):
     layer output and returns them in the original shape, like the reference.  Unlike the
     reference, the gate projection is not a separate GEMM: the router kernel computes it while it
     reads the tokens.  ``fuse_gate=False`` restores the separate ``F.linear``, which batches of up to
-    ``few_token_limit`` tokens take too.
+    ``few_token_limit`` tokens take too (a library GEMM before the layer's two kernels).
     """
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,

@@ -439,7 +439,8 @@ int b200moe_paged_schedule(const int32_t* context_lens, const int32_t* new_lens,
  *   new codes <- e4m3(x / scale), round to nearest even; NaN stays NaN, infinities become +-448
  * A call that stores to a page's first slot begins the page anew: its old scale and codes count for
  * nothing.  Slots must be distinct, and the tokens of one page must follow one another in the call with
- * nothing but skipped entries between them.  head_dim must be 128.
+ * nothing but skipped entries between them (anything else is not found out: codes and scale of that page are then
+ * undefined).  head_dim must be 128, num_tokens at most 65535 * 256.
  *
  * b200moe_paged_attn_varlen_fp8 is b200moe_paged_attn_varlen over such caches; q rows are q_row_stride
  * elements apart (a multiple of 8), table rows table_row_stride.  Scores, softmax statistics and sums
